@@ -39,6 +39,8 @@ LIBRARIES = {
     "latent_attention": "latent_attention.cu",
     "recurrent": "recurrent.cu",
     "moe": "moe.cu",
+    "gemm_int8": "gemm_int8.cu",
+    "norm_gate": "norm_gate.cu",
     "diff_attention": "diff_attention.cu",
     "channel_scan": "channel_scan.cu",
     "bias_attention": "bias_attention.cu",
@@ -59,6 +61,8 @@ KERNEL_LIBRARIES = ["elementwise", "gemm_simt", "gemm_bf16", "attention_generic"
 EXTRA_SOURCES = {
     "host_runtime": ["host/dispatch.hpp"],
     "gemm_simt": ["per_device.h"],
+    "gemm_int8": ["int8_rows.cuh", "per_device.h"],
+    "norm_gate": ["int8_rows.cuh", "per_device.h"],
     "recurrent": ["portion_rounds.h", "per_device.h"],
     "channel_scan": ["portion_rounds.h", "per_device.h"],
     "executor": ["host/executor.hpp", "host/kernels.hpp", "host/dispatch.hpp"],

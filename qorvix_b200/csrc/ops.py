@@ -128,11 +128,17 @@ _ARGTYPES = {
     "qv_head_delta_block": [],
     "qv_head_delta_state_floats": [_I, _I, _I],
     "qv_head_delta_scan": [_V, _I, _V, _V, _V, _I, _V, _V, _L, _V, _V, _I, _I, _I, _I, _I, _I, _I, _V],
+    "qv_quantize_rows": [_V, _L, _V, _V, _L, _I, _V, _I, _I, _I, _V],
+    "qv_int8_packed_bytes": [_I, _I, _I],
+    "qv_pack_int8": [_V, _V, _L, _I, _I, _I, _V],
+    "qv_gemm_int8": [_V, _L, _I, _V, _L, _V, _V, _V, _I, _I, _I, _I, _V, _I, _I, _I, _F, _F, _V, _V],
+    "qv_linear_int8": [_V, _L, _I, _V, _L, _I, _V, _L, _V, _V, _V, _I, _I, _I, _I, _F, _F, _V, _V],
+    "qv_norm_gate_add": [_V, _V, _V, _L, _I, _V, _F, _V, _L, _I, _V, _V, _V, _F, _V, _L, _I, _V, _I, _I, _V],
     "qv_argmax": [_V, _V, _I, _I, _L, _V],
     "qv_argmax_ctas": [_I, _I],
     "qv_sample": [_V, _V, _I, _I, _L, _V, _V, _V, _V, _V, _V, _I, _V, _V, _V, _V],
 }
-_RESTYPES = {"qv_error_string": ctypes.c_char_p, "qv_packed_weight_bytes": c_longlong, "qv_gemm_bf16_split_slot_bytes": c_longlong,
+_RESTYPES = {"qv_error_string": ctypes.c_char_p, "qv_int8_packed_bytes": c_longlong, "qv_packed_weight_bytes": c_longlong, "qv_gemm_bf16_split_slot_bytes": c_longlong,
              "qv_linear_scan_state_floats": c_longlong, "qv_linear_scan_workspace_bytes": c_longlong, "qv_latent_tc_workspace_bytes": c_longlong, "qv_diff_partial_floats": c_longlong,
              "qv_channel_scan_state_floats": c_longlong, "qv_channel_delta_workspace_floats": c_longlong, "qv_head_delta_state_floats": c_longlong}
 _typed_libs = {}
@@ -1757,6 +1763,238 @@ def check_kernel_errors() -> None:
         if code:
             st["err"].zero_()
             raise KernelError(f"a tensor-core kernel on device {key} gave up waiting on a barrier (code {code})")
+
+
+# ------------------------------------------------------------------ 8-bit integers
+
+INT8_MAX_K = 131071                        # 128 * 128 * K must stay below 2^31: the products' sums are int32
+INT8_TILE_ROWS = (32, 64, 128, 256)
+
+
+class Int8Rows:
+    """Rows of 8-bit integers, each with a scale: values int8 [T, K] (row stride a multiple of 16, on 16 bytes), scale float32 [T]; the row
+    stands for values * scale."""
+    __slots__ = ("values", "scale")
+
+    def __init__(self, values, scale):
+        self.values, self.scale = values, scale
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def device(self):
+        return self.values.device
+
+
+class Int8Weight:
+    """A matrix [N, K] of 8-bit integers with a scale a row, or `experts` of them (0: one), laid out for the products (pack_int8)."""
+    __slots__ = ("packed", "scale", "n", "k", "experts")
+
+    def __init__(self, packed, scale, n: int, k: int, experts: int):
+        self.packed, self.scale, self.n, self.k, self.experts = packed, scale, n, k, experts
+
+    @property
+    def device(self):
+        return self.packed.device
+
+
+def _on_current(*tensors) -> None:
+    """All on the device that launches go to."""
+    _need_cuda(*tensors)
+    dev = _get_device() if _get_device is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise KernelError(f"kernel operands must live on the current CUDA device ({dev}), not on {t.device}")
+
+
+def int8_rows(tokens: int, k: int, device) -> Int8Rows:
+    """Room for `tokens` rows of k 8-bit integers."""
+    values = torch.empty((tokens, -(-k // 16) * 16), device=device, dtype=torch.int8)
+    return Int8Rows(values if k % 16 == 0 else values[:, :k], torch.empty(tokens, device=device, dtype=torch.float32))
+
+
+def _int8_rows_checked(rows: Int8Rows) -> Int8Rows:
+    v, s = rows.values, rows.scale
+    if v.dtype != torch.int8 or v.dim() != 2 or s.dtype != torch.float32 or s.shape != v.shape[:1] or not s.is_contiguous():
+        raise KernelError("8-bit rows are int8 [T, K] with a contiguous float32 scale [T]")
+    if v.stride(1) != 1 or (v.shape[0] > 1 and (v.stride(0) % 16 or v.stride(0) < v.shape[1])) or v.data_ptr() % 16:
+        raise KernelError("8-bit rows must start on 16 bytes (int8_rows makes such room)")
+    return rows
+
+
+def _ld(t) -> int:
+    """The row stride of a matrix; of a single row, whose stride says nothing, its width."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def quantize_rows(rows: Int8Rows, x, row_idx=None) -> None:
+    """rows[r] = x[r], or x[row_idx[r]], in 8 bits: values = round(127 x / max|x|) (the exact quotient; ties to the even one), scale =
+    max|x| / 127.  x float32 or bfloat16, rows may be strided.  A row of zeros has scale 0; one that holds an infinity or a NaN has scale
+    NaN; an index outside x's rows gives a row of zeros."""
+    _int8_rows_checked(rows)
+    _on_current(rows.values, rows.scale, x, row_idx)
+    T, K = rows.values.shape
+    if x.dim() != 2 or x.shape[1] != K or (K > 1 and x.stride(1) != 1):
+        raise KernelError(f"rows of {K} entries wanted, whole in memory, not {tuple(x.shape)} with strides {x.stride()}")
+    if row_idx is None:
+        if x.shape[0] != T:
+            raise KernelError(f"{x.shape[0]} rows do not fill {T}")
+    else:
+        _i32(row_idx, "row_idx")
+        if row_idx.numel() != T:
+            raise KernelError(f"{row_idx.numel()} row indices do not fill {T} rows")
+    if T == 0:
+        return
+    rc = _lib("gemm_int8").qv_quantize_rows(_ptr(rows.values), _ld16(rows.values), _ptr(rows.scale), _ptr(x), _ld(x), dt_code(x.dtype), _ptr(row_idx),
+                                            x.shape[0], T, K, _stream())
+    _check(rc, "quantize_rows")
+
+
+def _ld16(v) -> int:
+    """The row stride of 8-bit rows; of a single row the next multiple of 16."""
+    return v.stride(0) if v.shape[0] > 1 else -(-v.shape[1] // 16) * 16
+
+
+def pack_int8(values, scale) -> Int8Weight:
+    """The matrix values (int8 [N, K], or [E, N, K] for experts) with scale (float32 [N] or [E, N]) in the tiles the products read; a copy."""
+    _on_current(values, scale)
+    if values.dtype != torch.int8 or values.dim() not in (2, 3) or scale.dtype != torch.float32 or scale.shape != values.shape[:-1]:
+        raise KernelError("pack_int8 takes int8 values [N, K] or [E, N, K] and a float32 scale for each row")
+    experts = values.shape[0] if values.dim() == 3 else 0
+    n, k = values.shape[-2:]
+    if min(values.shape) < 1 or k > INT8_MAX_K:
+        raise KernelError(f"a matrix of {n} x {k} is not one the 8-bit products take (1 to {INT8_MAX_K} entries a row)")
+    values = values.contiguous()
+    lib = _lib("gemm_int8")
+    packed = torch.empty(lib.qv_int8_packed_bytes(max(experts, 1), n, k), device=values.device, dtype=torch.int8)
+    _check(lib.qv_pack_int8(_ptr(packed), _ptr(values), k, max(experts, 1), n, k, _stream()), "pack_int8")
+    return Int8Weight(packed, scale.reshape(-1).clone(), n, k, experts)
+
+
+def quantize_weight(w) -> Int8Weight:
+    """A float32 or bfloat16 matrix [N, K], or [E, N, K], in 8 bits: a scale for each output channel, from its largest entry (quantize_rows)."""
+    if w.dim() not in (2, 3):
+        raise KernelError("quantize_weight takes a matrix [N, K] or matrices [E, N, K]")
+    rows = int8_rows(w.numel() // max(w.shape[-1], 1), w.shape[-1], w.device)
+    quantize_rows(rows, w.reshape(-1, w.shape[-1]))
+    return pack_int8(rows.values.reshape(w.shape), rows.scale.reshape(w.shape[:-1]))
+
+
+def _int8_product(out, x, weight: Int8Weight, act: int, limit: float, slope: float, what: str) -> None:
+    n = weight.n if act < 0 else weight.n // 2
+    if weight.experts:
+        raise KernelError(f"{what} takes one matrix; experts' matrices go to moe_experts_int8")
+    if act >= 0 and (weight.n % 32 or act not in (GLU_SILU, GLU_GELU_TANH, GLU_CLAMPED)):
+        raise KernelError(f"{what}: gate and up rows alternate in groups of 16, and act is GLU_SILU, GLU_GELU_TANH or GLU_CLAMPED")
+    T, K = x.shape
+    if K != weight.k or out.dim() != 2 or out.shape[0] != T or out.shape[1] != n or (n > 1 and out.stride(1) != 1):
+        raise KernelError(f"{what}: rows {tuple(x.shape)} and a matrix of {weight.n} x {weight.k} do not give {tuple(out.shape)}")
+    if T > 1 and out.stride(0) < n:
+        raise KernelError(f"{what}: the output's rows overlap")
+    if T == 0:
+        return
+    lib = _lib("gemm_int8")
+    err = _ptr(_tc_buffers(out.device)["err"])
+    if isinstance(x, Int8Rows):
+        _int8_rows_checked(x)
+        _on_current(out, x.values, x.scale, weight.packed)
+        rc = lib.qv_gemm_int8(_ptr(out), _ld(out), dt_code(out.dtype), _ptr(x.values), _ld16(x.values), _ptr(x.scale), _ptr(weight.packed), _ptr(weight.scale),
+                              T, weight.n, K, 1, None, 0, 0, act, float(limit), float(slope), err, _stream())
+        _check(rc, what)
+        return
+    _on_current(out, x, weight.packed)
+    if K > 1 and x.stride(1) != 1:
+        raise KernelError(f"{what}: rows must be whole in memory, not strides {x.stride()}")
+    ld = -(-K // 16) * 16
+    room = torch.empty(T * (ld + 4), device=x.device, dtype=torch.int8)        # the rows in 8 bits, then their scales
+    q = room.data_ptr()
+    rc = lib.qv_linear_int8(_ptr(out), _ld(out), dt_code(out.dtype), _ptr(x), _ld(x), dt_code(x.dtype), q, ld, q + T * ld, _ptr(weight.packed),
+                            _ptr(weight.scale), T, weight.n, K, act, float(limit), float(slope), err, _stream())
+    _check(rc, what)
+    add_launches(1)
+
+
+def gemm_int8(out, x, weight: Int8Weight) -> None:
+    """out [T, N] (float32 or bfloat16) = x W^T in 8-bit integers: the whole sum of values times the token's scale times the channel's.  x:
+    Int8Rows, or float32 or bfloat16 rows [T, K], which are put into 8 bits first (quantize_rows)."""
+    _int8_product(out, x, weight, -1, 0.0, 0.0, "gemm_int8")
+
+
+def gemm_int8_glu(out, x, weight: Int8Weight, act: int = 0, limit: float = 0.0, slope: float = 0.0) -> None:
+    """out [T, N / 2] = act(gate) * up of a gate/up product whose matrix alternates 16 gate rows and the 16 up rows of the same features
+    (act, limit, slope: see glu_act); x as for gemm_int8."""
+    _int8_product(out, x, weight, int(act), limit, slope, "gemm_int8_glu")
+
+
+def moe_int8_tile_rows(rows: int, experts: int) -> int:
+    """Rows of a tile of grouped rows for the 8-bit experts' products: what the tile table (moe_group) is made for."""
+    want = -(-4 * rows // (3 * max(experts, 1)))
+    return 32 if want <= 32 else 64 if want <= 64 else 128 if want <= 128 else 256
+
+
+def moe_experts_int8(up, out, rows: Int8Rows, weight: Int8Weight, tiles, act: int = GLU_SILU, limit: float = 0.0, slope: float = 0.0, tile_rows: int = 0) -> None:
+    """The experts' products in 8-bit integers over rows in grouped order: up True: out [R, N / 2] = act(gate) * up (matrices as for
+    gemm_int8_glu), False: out [R, N] the products themselves; float32 or bfloat16.  tiles: moe_group's table, made for tiles of `tile_rows`
+    rows (moe_int8_tile_rows).  Rows that no tile lists are left as they were."""
+    n = weight.n // 2 if up else weight.n
+    _int8_rows_checked(rows)
+    _on_current(out, rows.values, rows.scale, weight.packed, tiles)
+    _i32(tiles, "tiles")
+    R, K = rows.shape
+    if not weight.experts or tile_rows not in INT8_TILE_ROWS:
+        raise KernelError("moe_experts_int8 takes experts' matrices and tiles of 32, 64, 128 or 256 rows")
+    if up and (weight.n % 32 or act not in (GLU_SILU, GLU_GELU_TANH, GLU_CLAMPED)):
+        raise KernelError("moe_experts_int8: gate and up rows alternate in groups of 16, and act is GLU_SILU, GLU_GELU_TANH or GLU_CLAMPED")
+    if K != weight.k or tuple(out.shape) != (R, n) or (n > 1 and out.stride(1) != 1) or (R > 1 and out.stride(0) < n):
+        raise KernelError(f"moe_experts_int8: rows {tuple(rows.shape)} and matrices of {weight.n} x {weight.k} do not give {tuple(out.shape)}")
+    if tiles.numel() % 3:
+        raise KernelError("the tile table holds three numbers a tile")
+    if R == 0 or tiles.numel() == 0:
+        return
+    rc = _lib("gemm_int8").qv_gemm_int8(_ptr(out), _ld(out), dt_code(out.dtype), _ptr(rows.values), _ld16(rows.values), _ptr(rows.scale), _ptr(weight.packed),
+                                        _ptr(weight.scale), R, weight.n, K, weight.experts, _ptr(tiles), tiles.numel() // 3, tile_rows, int(act) if up else -1,
+                                        float(limit), float(slope), _ptr(_tc_buffers(out.device)["err"]), _stream())
+    _check(rc, "moe_experts_int8")
+
+
+def norm_gate_add(residual, y=None, post_weight=None, post_eps: float = 0.0, gate=None, gate_bias=None, scale=None, next_weight=None, next_eps: float = 0.0,
+                  out=None, into=None) -> None:
+    """What lies between two sublayers, in one pass: z = y, normed (y / rms(y) * post_weight) if there is a post_weight, times
+    sigmoid(gate + gate_bias) if there is a gate, times scale if there is one; residual += z (or into = residual + z, with residual left as it
+    is); out = the new residual, normed with next_weight if there is one.  residual and into float32 [T, d] contiguous; y and gate [T, d]
+    float32 or bfloat16 (rows may be strided); the weights, gate_bias and scale float32 [d]; out None, float32, bfloat16 (rows may be strided)
+    or Int8Rows (the bfloat16 rows in 8 bits, see quantize_rows)."""
+    rows8 = isinstance(out, Int8Rows)
+    if rows8:
+        _int8_rows_checked(out)
+    o = out.values if rows8 else out
+    _on_current(residual, y, post_weight, gate, gate_bias, scale, next_weight, o, into)
+    T, d = residual.shape
+    into = residual if into is None else into
+    if residual.dtype != torch.float32 or not residual.is_contiguous() or into.dtype != torch.float32 or not into.is_contiguous() or into.shape != residual.shape:
+        raise KernelError("the residual stream is contiguous float32 [T, d]")
+    if into is not residual and into.data_ptr() != residual.data_ptr() and abs(into.data_ptr() - residual.data_ptr()) < residual.nbytes:
+        raise KernelError("the new residual stream lies partly over the old one")
+    for t, name in ((y, "y"), (gate, "gate"), (o, "out")):
+        if t is not None and (tuple(t.shape) != (T, d) or (d > 1 and t.stride(1) != 1)):
+            raise KernelError(f"{name} must be [{T}, {d}] with whole rows, not {tuple(t.shape)} with strides {t.stride()}")
+    for t, name in ((post_weight, "post_weight"), (gate_bias, "gate_bias"), (scale, "scale"), (next_weight, "next_weight")):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != d or not t.is_contiguous()):
+            raise KernelError(f"{name} must be contiguous float32 [{d}]")
+    if y is None and (post_weight is not None or gate is not None or scale is not None):
+        raise KernelError("a norm, a gate or a scale needs a y")
+    if (gate is None and gate_bias is not None) or (out is None and next_weight is not None):
+        raise KernelError("a gate's bias needs a gate, and the next norm's weight rows to write")
+    if T == 0 or d == 0 or (y is None and out is None and into is residual):
+        return
+    rc = _lib("norm_gate").qv_norm_gate_add(
+        _ptr(residual), _ptr(into), _ptr(y), _ld(y) if y is not None else d, dt_code(y.dtype) if y is not None else F32, _ptr(post_weight), float(post_eps),
+        _ptr(gate), _ld(gate) if gate is not None else d, dt_code(gate.dtype) if gate is not None else F32, _ptr(gate_bias), _ptr(scale), _ptr(next_weight),
+        float(next_eps), _ptr(o), (_ld16(o) if rows8 else _ld(o)) if o is not None else d, 2 if rows8 else dt_code(o.dtype) if o is not None else F32,
+        _ptr(out.scale) if rows8 else None, T, d, _stream())
+    _check(rc, "norm_gate_add")
 
 
 # ------------------------------------------------------------------ attention
