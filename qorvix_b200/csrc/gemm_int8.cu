@@ -237,26 +237,78 @@ __global__ void __launch_bounds__(192) int8_product_kernel(const __grid_constant
 }
 
 // ---------------------------------------------------------------- rows in 8 bits
-template <typename T>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(int8_t* __restrict__ q, long long ld_q, float* __restrict__ scale, const T* __restrict__ x,
-                                                            long long ld_x, const int* __restrict__ row_idx, int rows_in, int K) {
-  __shared__ uint32_t red[33];
+// One read and one write of the row are all it cannot do without, so a row stays in registers between its maximum and its rounding: VECS
+// pieces of 16 bytes a thread, all asked for at once.  A row has a block of its own, whose size goes by the row's length; rows longer than
+// VECS pieces of 1,024 threads are read twice (LONG).  ALIGNED: pieces lie on 16 bytes; else their entries are read one by one.
+template <typename T> struct Piece { static constexpr int N = 16 / (int)sizeof(T); };
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void load_piece(float (&f)[Piece<T>::N], const T* x, int k, int K) {
+  constexpr int N = Piece<T>::N;
+  if (ALIGNED && k + N <= K) {
+    const uint4 v = *(const uint4*)(x + k);
+    const T* e = (const T*)&v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = to_f(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = k + i < K ? to_f(x[k + i]) : 0.f;
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_piece(int8_t* q, const float (&f)[N], const Int8Scale& s, int k, int K) {
+  uint32_t w[N / 4];
+  int8_pack<N>(f, s, w);
+  if (k + N <= K) {
+    if (N == 8) *(uint2*)(q + k) = make_uint2(w[0], w[N / 4 - 1]);
+    else *(uint32_t*)(q + k) = w[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (k + i < K) q[k + i] = (int8_t)(w[i / 4] >> (8 * (i & 3)));
+  }
+}
+
+template <typename T, int VECS, bool ALIGNED, bool LONG>
+__global__ void __launch_bounds__(1024) quantize_rows_kernel(int8_t* __restrict__ q, long long ld_q, float* __restrict__ scale, const T* __restrict__ x,
+                                                             long long ld_x, const int* __restrict__ row_idx, int rows_in, int K) {
+  constexpr int N = Piece<T>::N;
+  __shared__ uint32_t red[32];
   pdl_wait();
   pdl_launch_dependents();
-  const int r = blockIdx.x;
+  const int r = blockIdx.x, step = blockDim.x * N;
   const int src = row_idx ? row_idx[r] : r;
   const bool there = (unsigned)src < (unsigned)rows_in;      // an index outside the rows: a row of zeros
   const T* xr = x + (size_t)(there ? src : 0) * ld_x;
+  const int n = there ? K : 0;
+  int8_t* o = q + (size_t)r * ld_q;
+  float f[VECS][N];
   uint32_t top = 0;
-  if (there)
-    for (int i = threadIdx.x; i < K; i += blockDim.x) {
-      const uint32_t b = __float_as_uint(to_f(xr[i])) & 0x7fffffffu;
-      top = b > top ? b : top;
+  if (LONG) {
+    for (int k = threadIdx.x * N; k < n; k += step) {
+      load_piece<T, ALIGNED>(f[0], xr, k, n);
+#pragma unroll
+      for (int i = 0; i < N; ++i) top = max(top, int8_bits(f[0][i]));
     }
+  } else {
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) load_piece<T, ALIGNED>(f[v], xr, threadIdx.x * N + v * step, n);
+#pragma unroll
+    for (int v = 0; v < VECS; ++v)
+#pragma unroll
+      for (int i = 0; i < N; ++i) top = max(top, int8_bits(f[v][i]));
+  }
   const Int8Scale s = int8_scale(int8_block_top(top, red));
   if (threadIdx.x == 0) scale[r] = s.scale;
-  int8_t* o = q + (size_t)r * ld_q;
-  for (int i = threadIdx.x; i < K; i += blockDim.x) o[i] = (int8_t)(there ? int8_of(to_f(xr[i]), s) : 0);
+  if (LONG) {
+    for (int k = threadIdx.x * N; k < K; k += step) {
+      load_piece<T, ALIGNED>(f[0], xr, k, n);
+      store_piece<N>(o, f[0], s, k, K);
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < VECS; ++v)
+      if (threadIdx.x * N + v * step < K) store_piece<N>(o, f[v], s, threadIdx.x * N + v * step, K);
+  }
 }
 
 // ---------------------------------------------------------------- packing
@@ -331,13 +383,30 @@ extern "C" int qv_pack_int8(void* out, const int8_t* values, long long ld, int E
   return qv_launch_status();
 }
 
-// q [T, K] (row stride ld_q) and scale [T] of the rows of x (row stride ld_x, rows_in of them), row r from row_idx[r] where row_idx is given.
+// q [T, K] (row stride ld_q, a multiple of 16, on 16 bytes) and scale [T] of the rows of x (row stride ld_x, rows_in of them), row r from
+// row_idx[r] where row_idx is given.
 extern "C" int qv_quantize_rows(int8_t* q, long long ld_q, float* scale, const void* x, long long ld_x, int x_dt, const int* row_idx, int rows_in, int T, int K,
                                 void* stream) {
   if (T <= 0) return 0;
-  if (K <= 0 || ld_q < K || ld_x < K || (!row_idx && rows_in < T)) return QV_ERR_UNSUPPORTED;
-  QV_DISPATCH_DT(x_dt, TX, return qv_launch(quantize_rows_kernel<TX>, dim3(T), dim3(256), 0, (cudaStream_t)stream, q, ld_q, scale, (const TX*)x, ld_x, row_idx,
-                                            rows_in, K));
+  if (K <= 0 || ld_q < K || ((uintptr_t)q & 15) || (ld_q & 15) || ld_x < K || (!row_idx && rows_in < T)) return QV_ERR_UNSUPPORTED;
+  cudaStream_t st = (cudaStream_t)stream;
+#define QUANTIZE(VECS, ALIGNED, LONG, THREADS)                                                                                                          \
+  return qv_launch(quantize_rows_kernel<TX, VECS, ALIGNED, LONG>, dim3(T), dim3(THREADS), 0, st, q, ld_q, scale, (const TX*)x, ld_x, row_idx, rows_in, K)
+#define QUANTIZE_AS(ALIGNED)                                                             \
+  do {                                                                                   \
+    if (pieces > 4096) QUANTIZE(1, ALIGNED, true, 1024);                                 \
+    if (few && pieces <= 1024) QUANTIZE(1, ALIGNED, false, (pieces + 31) / 32 * 32);     \
+    if (pieces <= 512) QUANTIZE(2, ALIGNED, false, (pieces + 63) / 64 * 32);             \
+    QUANTIZE(4, ALIGNED, false, (pieces + 127) / 128 * 32);                              \
+  } while (0)
+  QV_DISPATCH_DT(x_dt, TX, {
+    const int pieces = (K + Piece<TX>::N - 1) / Piece<TX>::N;
+    const bool few = T <= 2 * sms_of_device();
+    if (((uintptr_t)x & 15) == 0 && (ld_x * sizeof(TX)) % 16 == 0) QUANTIZE_AS(true);
+    QUANTIZE_AS(false);
+  });
+#undef QUANTIZE_AS
+#undef QUANTIZE
 }
 
 // out [rows, N] (act < 0) or [rows, N / 2] (a gated product, act a GluAct kind; N a multiple of 32) of x [rows, K] (8-bit, row stride ld_x, a multiple

@@ -32,26 +32,43 @@ __device__ __noinline__ float int8_border(float x, float v, float top) {
   return copysignf(r, x);
 }
 
-__device__ __forceinline__ int int8_of(float x, const Int8Scale& s) {
-  x *= s.pre;
-  const float v = x * s.inv;
-  float r = rintf(v);
-  if (fabsf(v - r) > 0.4999f) r = int8_border(x, v, s.top);
-  return s.live ? (int)r : 0;
+// Entries of a row as bytes, N of them (a multiple of 4) packed in words.  t = v + 1.5 2^23 holds round(v) in its low bits; v - round(v) says
+// how near the border lies, and the whole group is looked at once.
+template <int N>
+__device__ __forceinline__ void int8_pack(const float (&x)[N], const Int8Scale& s, uint32_t (&out)[N / 4]) {
+  constexpr float MAGIC = 12582912.f;
+  float t[N], far = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float xi = x[i] * s.pre;
+    t[i] = fmaf(xi, s.inv, MAGIC);
+    far = fmaxf(far, fabsf(fmaf(xi, s.inv, MAGIC - t[i])));
+  }
+  if (far > 0.4999f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float xi = x[i] * s.pre, v = xi * s.inv;
+      if (fabsf(fmaf(xi, s.inv, MAGIC - t[i])) > 0.4999f) t[i] = MAGIC + int8_border(xi, v, s.top);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const uint32_t lo = __byte_perm(__float_as_uint(t[i]), __float_as_uint(t[i + 1]), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(t[i + 2]), __float_as_uint(t[i + 3]), 0x0040);
+    out[i / 4] = s.live ? __byte_perm(lo, hi, 0x5410) : 0u;
+  }
 }
 
-__device__ __forceinline__ uint32_t int8_pack4(int a, int b, int c, int d) {
-  return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
-}
+// The largest magnitude's bits: of finite and infinite numbers and NaN alike, ordered as unsigned numbers, NaN on top.
+__device__ __forceinline__ uint32_t int8_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// The largest of the magnitudes `bits` (of finite and infinite numbers and NaN alike: as unsigned numbers they are ordered, NaN on top),
-// over the block.
-__device__ __forceinline__ float int8_block_top(uint32_t bits, uint32_t* red /* >= 33 */) {
+// The largest of `bits` over the block's threads, as a float.
+__device__ __forceinline__ float int8_block_top(uint32_t bits, uint32_t* red /* >= 32 */) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = (blockDim.x + 31) >> 5;
   bits = __reduce_max_sync(0xffffffffu, bits);
+  if (nwarp == 1) return __uint_as_float(bits);
   __syncthreads();
   if (lane == 0) red[warp] = bits;
   __syncthreads();
-  uint32_t t = lane < nwarp ? red[lane] : 0u;
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, t));
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, lane < nwarp ? red[lane] : 0u));
 }
