@@ -9,10 +9,6 @@
 // row r at chunk c ^ (r % 8)), zero where the matrix ends.  It is the 128-row operand and the token rows are the narrow one, so that a
 // thread of the epilogue holds one channel of many tokens, rows are padded to 16 only, and dense and grouped products are one kernel.
 //
-// One CTA per SM walks over items (a tile of rows, a block of 128 channels):
-//   warp 0      weights by contiguous bulk copies, rows by TMA, through a ring of STAGES
-//   warp 1      tcgen05.mma, accumulators double-buffered in tensor memory
-//   warps 2..5  epilogue of the item before: scales, activation, stores
 // Every wait is bounded; one that gives up records a code and the CTA winds down.
 #include "int8_rows.cuh"
 #include "per_device.h"
@@ -23,9 +19,9 @@
 
 namespace {
 
-// Instruction descriptor, kind::i8: D int32, A and B signed 8-bit, both K-major, 128 x n.
-__device__ __forceinline__ uint32_t umma_idesc_i8(int n) {
-  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+// Instruction descriptor, kind::i8: D int32, A and B signed 8-bit, both K-major, m x n.
+__device__ __forceinline__ uint32_t umma_idesc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -47,6 +43,8 @@ struct Int8Args {
   int rows, row_tiles, bn;            // dense: rows in all, tiles of them, rows of a tile (a multiple of 16); grouped: row_tiles is the table's length
   int box;                            // rows of a TMA box
   int N, K;
+  int splits, kb_per_split;           // few rows: CTAs that share a block of channels, and the k blocks of each
+  int mine_shift;                     // and, as a power of two, the columns of which each adds up the sums
   GluAct glu;
 };
 
@@ -90,23 +88,225 @@ template <typename TO> __device__ __forceinline__ float gated(float g, float u, 
   return g / (1.f + expf(-arg)) * u;
 }
 
-// GLU: a gated product.  TO: the output's type.  RT: rows of a tile at most.
+// ---------------------------------------------------------------- many rows, and rows grouped by expert
+// Two CTAs of a cluster, on neighbouring SMs, work on 256 channels x up to 256 rows: each holds 128 channels of the matrix and half of the
+// rows in its shared memory, and one instruction (cta_group::2) multiplies all channels with all rows, so an SM takes in 32 KB for the products
+// that it would have to take in 48 KB for by itself.  What an SM takes in sets the pace of such a kernel, not the products.  The pairs
+// walk over items (a tile of rows, a block of 256 channels):
+//   warp 0      weights and rows by TMA through a ring of STAGES; both CTAs' copies report to the first CTA's barrier
+//   warp 1      of the first CTA: tcgen05.mma, accumulators double-buffered in tensor memory
+//   warps 2..9  epilogue of the item before: scales, activation, stores; two warps share the channels of a quarter of tensor memory and
+//               take groups of 32 rows in turn
+// GLU: a gated product.  TO: the output's type.  RT: rows of a tile at most (a multiple of 32).
+#define PAIR_THREADS 320
+__device__ __forceinline__ uint32_t of_first(const void* p) {      // the address of the same variable in the cluster's first CTA
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {       // arrives on the barrier of both CTAs when the products issued so far are done
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+
 template <bool GLU, typename TO, int RT, int STAGES>
-__global__ void __launch_bounds__(192) int8_product_kernel(const __grid_constant__ CUtensorMap map_x, const Int8Args p) {
+__global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                                                                 const Int8Args p) {
   extern __shared__ uint8_t smem_raw[];
-  constexpr int STAGE_BYTES = W_TILE_BYTES + RT * QK;
-  constexpr int TMEM_COLS = 2 * RT < 32 ? 32 : 2 * RT;
+  constexpr int STAGE_BYTES = W_TILE_BYTES + RT / 2 * QK;
+  constexpr int TMEM_COLS = 2 * RT;
   uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  float* scales = (float*)(ring + STAGES * STAGE_BYTES);       // [4 warps][RT]: the rows' scales
-  uint64_t* full = (uint64_t*)(scales + 4 * RT);
+  constexpr int SCALES = RT < 64 ? 32 : RT / 2;
+  float* scales = (float*)(ring + STAGES * STAGE_BYTES);       // [8 warps][SCALES]: the scales of the rows that a warp takes
+  uint64_t* full = (uint64_t*)(scales + 8 * SCALES);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;               // [2]
   uint64_t* acc_empty = acc_full + 2;                // [2]
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1;                   // within the pair
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 128); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 16); }      // 8 epilogue warps of either CTA
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");    // the other CTA's barriers are set up
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();                                        // the rows, the tile table and the output belong to the kernels ahead until here
+  const int NT = (p.N + BM - 1) / BM, NP = (NT + 1) / 2, KT = (p.K + QK - 1) / QK;
+  const int items = p.row_tiles * NP, first = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp == 0) {
+    const bool leader = elect_one();
+    int it = 0;
+    bool ok = true;
+    for (int item = first; ok && item < items; item += pairs) {
+      const Item w = item_at(p, item, NP);
+      if (w.e < 0) break;
+      const int half = ((w.rows + 31) & ~31) >> 1;             // rows of either CTA
+      const int boxes = (half + p.box - 1) / p.box;
+      const int block = 2 * w.fb + rank < NT ? 2 * w.fb + rank : NT - 1;       // (a last block without a second half: its sums go nowhere)
+      const int w_row = ((w.e * NT + block) * KT) * BM, x_row = w.row0 + rank * half;
+      for (int kb = 0; kb < KT; ++kb, ++it) {
+        const int s = it % STAGES;
+        if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, p.err, 61)) { ok = false; break; }
+        if (leader) {
+          uint8_t* dst = ring + s * STAGE_BYTES;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * (W_TILE_BYTES + boxes * p.box * QK));
+          const uint32_t bar = of_first(&full[s]);
+          tma_load_pair(dst, &map_w, bar, 0, w_row + kb * BM);
+          for (int x = 0; x < boxes; ++x) tma_load_pair(dst + W_TILE_BYTES + x * p.box * QK, &map_x, bar, kb * QK, x_row + x * p.box);
+        }
+        __syncwarp();
+      }
+    }
+    // after a wait that gave up: the copies in flight land before either CTA's shared memory goes to another
+    if (!ok && rank == 0)
+      for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, p.err, 65);
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool leader = elect_one();               // the whole warp walks the loop and waits, an elected lane issues
+      int it = 0, local = 0;
+      bool ok = true;
+      for (int item = first; ok && item < items; item += pairs, ++local) {
+        const Item w = item_at(p, item, NP);
+        if (w.e < 0) break;
+        const uint32_t idesc = umma_idesc_i8(2 * BM, (w.rows + 31) & ~31);
+        const int b = local & 1;
+        ok = mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, p.err, 64);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(b * RT);
+        for (int kb = 0; kb < KT; ++kb, ++it) {
+          const int s = it % STAGES;
+          ok = mbar_wait(&full[s], (it / STAGES) & 1, p.err, 62);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(ring + s * STAGE_BYTES);
+          const uint64_t da = umma_desc(a_addr), db = umma_desc(a_addr + W_TILE_BYTES);
+          if (leader) {
+#pragma unroll
+            for (int kk = 0; kk < QK / 32; ++kk)     // 32 entries of k a product: 32 bytes, 2 descriptor units
+              umma_i8_pair(d_tmem, da + 2 * kk, db + 2 * kk, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            commit_pair(&empty[s]);
+          }
+          __syncwarp();
+        }
+        if (leader) commit_pair(&acc_full[b]);
+        __syncwarp();
+      }
+    }
+  } else {
+    const int q = warp & 3, turn = (warp - 2) >> 2;            // tensor memory lanes 32 q .. + 31; groups of 32 rows: turn, turn + 2, ...
+    float* xs = scales + (warp - 2) * SCALES;
+    const uint32_t done[2] = {of_first(&acc_empty[0]), of_first(&acc_empty[1])};
+    int local = 0;
+    for (int item = first; item < items; item += pairs, ++local) {
+      const Item w = item_at(p, item, NP);
+      if (w.e < 0) break;
+      const int ch0 = (2 * w.fb + rank) * BM + q * 32;         // this warp's channels
+      const float ws = ch0 + lane < p.N ? p.w_scale[(size_t)w.e * p.N + ch0 + lane] : 0.f;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < SCALES; i += 32) {
+        const int row = 2 * i + turn * 32 + lane;
+        xs[i + lane] = row < w.rows ? p.x_scale[w.row0 + row] : 0.f;
+      }
+      __syncwarp();
+      const int b = local & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[b], (local >> 1) & 1, p.err, 63))) break;     // (the MMA warp then gives up too)
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * RT);
+      const int feat = GLU ? (ch0 >> 1) + (lane & 15) : ch0 + lane;
+      const bool there = GLU ? 2 * feat < p.N : feat < p.N;
+      TO* out = (TO*)p.out + (size_t)w.row0 * p.ld_out + feat;
+#pragma unroll 1
+      for (int c0 = turn * 32; c0 < w.rows; c0 += 64) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c0, r);
+        const float* sc = xs + (c0 >> 6) * 32;
+        tmem_wait_ld();
+        if (GLU) {
+          // a lane of the lower half gives its gate value of the odd row for the up value of the even row
+          const int up = lane >> 4;
+          TO* o = out + (size_t)(c0 + up) * p.ld_out;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float a = (float)(int)r[j] * sc[j] * ws, c = (float)(int)r[j + 1] * sc[j + 1] * ws;
+            const float got = __shfl_xor_sync(0xffffffffu, up ? a : c, 16);
+            const float g = up ? got : a, u = up ? c : got;
+            if (c0 + j + up < w.rows && there) o[(size_t)j * p.ld_out] = from_f<TO>(gated<TO>(g, u, p.glu));
+          }
+        } else if (there) {
+          TO* o = out + (size_t)c0 * p.ld_out;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j < w.rows) o[(size_t)j * p.ld_out] = from_f<TO>((float)(int)r[j] * sc[j] * ws);
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(done[b]) : "memory");
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");    // neither CTA's shared or tensor memory is in the other's use any more
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+// A step of few tokens is bound by the matrix' bytes, so that all SMs have to ask for weights at once, and from the start: a block of 128
+// channels is shared along k by the CTAs of a cluster (grid z), each with a ring of its own, and the first weights are asked for before the
+// wait for the kernel ahead (a packed matrix lies still: qv_pack_int8 lets no kernel start before its end).  The CTAs hand their int32 sums
+// to one another through distributed shared memory: CTA s adds up columns s, s + splits, ... of all of them, scales and stores these; whole
+// sums have no order, so splits change no bit.
+template <bool GLU, typename TO, int BN, int STAGES>
+__global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ CUtensorMap map_x, const Int8Args p) {
+  extern __shared__ uint8_t smem_raw[];
+  constexpr int STAGE_BYTES = W_TILE_BYTES + BN * QK;
+  constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
+  uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = (uint64_t*)(ring + STAGES * STAGE_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* accum = empty + STAGES;
+  uint32_t* tmem_slot = (uint32_t*)(accum + 1);
+  __shared__ float xs[BN];                                     // the rows' scales
+  int* sums = (int*)(ring + STAGES * STAGE_BYTES + 256);       // [splits][columns of this CTA / 4][128 channels][4]: what the cluster hands this CTA
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int KT = (p.K + QK - 1) / QK;
+  const int split = blockIdx.z, kb0 = split * p.kb_per_split;
+  const int num_kb = KT - kb0 < p.kb_per_split ? KT - kb0 : p.kb_per_split;
+  const int row0 = blockIdx.y * BN, rows = p.rows - row0 < BN ? p.rows - row0 : BN;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(accum, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -119,116 +319,129 @@ __global__ void __launch_bounds__(192) int8_product_kernel(const __grid_constant
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_launch_dependents();
-  pdl_wait();                                        // the rows, the tile table and the output belong to the kernels ahead until here
-  const int NT = (p.N + BM - 1) / BM, KT = (p.K + QK - 1) / QK;
-  const int items = p.row_tiles * NT;
+  if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");      // met ahead of the first store into another CTA
 
   if (warp == 0) {
     const bool leader = elect_one();
-    int it = 0;
-    bool ok = true;
-    for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const Item w = item_at(p, item, NT);
-      if (w.e < 0) break;
-      const int boxes = (w.rows + p.box - 1) / p.box;
-      const uint8_t* src = p.w + ((size_t)w.e * NT + w.fb) * KT * W_TILE_BYTES;
-      for (int kb = 0; kb < KT; ++kb, ++it) {
-        const int s = it % STAGES;
-        if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, p.err, 61)) { ok = false; break; }
-        if (leader) {
-          uint8_t* dst = ring + s * STAGE_BYTES;
-          mbar_expect_tx(&full[s], W_TILE_BYTES + boxes * p.box * QK);
-          bulk_load_1d(dst, src + (size_t)kb * W_TILE_BYTES, &full[s], W_TILE_BYTES);
-          for (int x = 0; x < boxes; ++x) tma_load_2d(dst + W_TILE_BYTES + x * p.box * QK, &map_x, &full[s], kb * QK, w.row0 + x * p.box);
-        }
-        __syncwarp();
+    const uint8_t* w = p.w + ((size_t)blockIdx.x * KT + kb0) * W_TILE_BYTES;
+    const int pre = num_kb < STAGES ? num_kb : STAGES;
+    if (leader)
+      for (int kb = 0; kb < pre; ++kb) {
+        mbar_expect_tx(&full[kb], STAGE_BYTES);
+        bulk_load_1d(ring + kb * STAGE_BYTES, w + (size_t)kb * W_TILE_BYTES, &full[kb], W_TILE_BYTES);
       }
+    __syncwarp();
+    pdl_wait();
+    if (leader)
+      for (int kb = 0; kb < pre; ++kb) tma_load_2d(ring + kb * STAGE_BYTES + W_TILE_BYTES, &map_x, &full[kb], (kb0 + kb) * QK, row0);
+    __syncwarp();
+    int kb = pre;
+    for (; kb < num_kb; ++kb) {
+      const int s = kb % STAGES;
+      if (!mbar_wait(&empty[s], ((kb / STAGES) & 1) ^ 1, p.err, 61)) break;
+      if (leader) {
+        uint8_t* dst = ring + s * STAGE_BYTES;
+        mbar_expect_tx(&full[s], STAGE_BYTES);
+        bulk_load_1d(dst, w + (size_t)kb * W_TILE_BYTES, &full[s], W_TILE_BYTES);
+        tma_load_2d(dst + W_TILE_BYTES, &map_x, &full[s], (kb0 + kb) * QK, row0);
+      }
+      __syncwarp();
     }
-    // after a wait that gave up: the copies in flight land before the CTA's shared memory goes to another
-    if (!ok)
-      for (int i = it < STAGES ? 0 : it - STAGES; i < it; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, p.err, 65);
+    if (kb < num_kb)                                 // gave up: the copies in flight land first
+      for (int i = kb < STAGES ? 0 : kb - STAGES; i < kb; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, p.err, 65);
   } else if (warp == 1) {
-    const bool leader = elect_one();                 // the whole warp walks the loop and waits, an elected lane issues
-    int it = 0, local = 0;
-    bool ok = true;
-    for (int item = blockIdx.x; ok && item < items; item += gridDim.x, ++local) {
-      const Item w = item_at(p, item, NT);
-      if (w.e < 0) break;
-      const uint32_t idesc = umma_idesc_i8((w.rows + 15) & ~15);
-      const int b = local & 1;
-      ok = mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1, p.err, 64);
-      if (!ok) break;
+    const bool leader = elect_one();
+    const uint32_t idesc = umma_idesc_i8(BM, BN);
+    for (int kb = 0; kb < num_kb; ++kb) {
+      const int s = kb % STAGES;
+      if (!mbar_wait(&full[s], (kb / STAGES) & 1, p.err, 62)) break;
       tc_fence_after();
-      const uint32_t d_tmem = tmem_base + (uint32_t)(b * RT);
-      for (int kb = 0; kb < KT; ++kb, ++it) {
-        const int s = it % STAGES;
-        ok = mbar_wait(&full[s], (it / STAGES) & 1, p.err, 62);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t a_addr = smem_u32(ring + s * STAGE_BYTES);
-        const uint64_t da = umma_desc(a_addr), db = umma_desc(a_addr + W_TILE_BYTES);
-        if (leader) {
+      const uint32_t a_addr = smem_u32(ring + s * STAGE_BYTES);
+      const uint64_t da = umma_desc(a_addr), db = umma_desc(a_addr + W_TILE_BYTES);
+      if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < QK / 32; ++kk)       // 32 entries of k a product: 32 bytes, 2 descriptor units
-            umma_i8(d_tmem, da + 2 * kk, db + 2 * kk, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&empty[s]);
-        }
-        __syncwarp();
+        for (int kk = 0; kk < QK / 32; ++kk) umma_i8(tmem_base, da + 2 * kk, db + 2 * kk, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&empty[s]);
       }
-      if (leader) umma_commit(&acc_full[b]);
       __syncwarp();
     }
-  } else {
-    const int q = warp & 3;                          // tensor memory lanes 32 q .. + 31
-    float* xs = scales + q * RT;
-    int local = 0;
-    for (int item = blockIdx.x; item < items; item += gridDim.x, ++local) {
-      const Item w = item_at(p, item, NT);
-      if (w.e < 0) break;
-      const int ch = w.fb * BM + q * 32 + lane;      // this thread's channel
-      const float ws = ch < p.N ? p.w_scale[(size_t)w.e * p.N + ch] : 0.f;
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < RT; i += 32)
-        if (i + lane < RT) xs[i + lane] = i + lane < w.rows ? p.x_scale[w.row0 + i + lane] : 0.f;
-      __syncwarp();
-      const int b = local & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[b], (local >> 1) & 1, p.err, 63))) break;     // (the MMA warp then gives up too)
-      tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * RT);
-      const int feat = GLU ? w.fb * 64 + q * 16 + (lane & 15) : ch;
-      const bool there = GLU ? 2 * feat < p.N : ch < p.N;
-      TO* out = (TO*)p.out + (size_t)w.row0 * p.ld_out + feat;
+    if (leader) umma_commit(accum);
+    __syncwarp();
+  }
+  const int q = warp & 3, ch0 = blockIdx.x * BM + q * 32;
+  const int feat = GLU ? (ch0 >> 1) + (lane & 15) : ch0 + lane;
+  const bool there = warp >= 2 && (GLU ? 2 * feat < p.N : feat < p.N);
+  TO* out = (TO*)p.out + (size_t)row0 * p.ld_out + feat;
+  float ws = 0.f;
+  // a column's scaled sums to the output: all lanes of an epilogue warp are here
+  auto finish = [&](int c, int sum) {
+    const float v = (float)sum * xs[c] * ws;
+    if (GLU) {
+      const float other = __shfl_xor_sync(0xffffffffu, v, 16);
+      if (lane < 16 && there) out[(size_t)c * p.ld_out] = from_f<TO>(gated<TO>(v, other, p.glu));
+    } else if (there) {
+      out[(size_t)c * p.ld_out] = from_f<TO>(v);
+    }
+  };
+  bool ok = true;
+  if (warp >= 2) {
+    pdl_wait();                                      // the rows' scales are the kernel's ahead, and the output may still be in its use
+    if (ch0 + lane < p.N) ws = p.w_scale[ch0 + lane];
+    const int te = threadIdx.x - 64;
+    if (te < BN) xs[te] = te < rows ? p.x_scale[row0 + te] : 0.f;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    ok = __all_sync(0xffffffffu, mbar_wait(accum, 0, p.err, 63));
+    tc_fence_after();
+  }
+  const int shift = p.mine_shift, mine = 1 << shift;           // columns a CTA adds up: 4 or more
+  if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  if (warp >= 2 && ok) {
+    const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
+    const uint32_t to = smem_u32(sums) + (uint32_t)(((split << (shift - 2)) * BM + q * 32 + lane) * 16);
 #pragma unroll 1
-      for (int c0 = 0; c0 < w.rows; c0 += 16) {
-        uint32_t r[16];
-        tmem_ld16(taddr + c0, r);
-        tmem_wait_ld();
-        float v[16];
+    for (int c0 = 0; c0 < rows; c0 += 16) {
+      uint32_t r[16];
+      tmem_ld16(taddr + c0, r);
+      tmem_wait_ld();
+      if (p.splits == 1) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = (float)(int)r[j] * xs[c0 + j] * ws;
-        if (GLU) {
-          // a lane of the lower half gives its gate value of the odd row for the up value of the even row
-          const int up = lane >> 4;
+        for (int j = 0; j < 16; ++j)
+          if (c0 + j < rows) finish(c0 + j, (int)r[j]);
+      } else {
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            const float got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + 1], 16);
-            const float g = up ? got : v[j], u = up ? v[j + 1] : got;
-            const int row = c0 + j + up;
-            if (row < w.rows && there) out[(size_t)row * p.ld_out] = from_f<TO>(gated<TO>(g, u, p.glu));
+        for (int j = 0; j < 16; j += 4) {
+          const int c = c0 + j;
+          if (c < rows) {
+            uint32_t remote;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(to + (uint32_t)(((c & (mine - 1)) >> 2) * BM * 16)), "r"(c >> shift));
+            asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "r"(r[j]), "r"(r[j + 1]), "r"(r[j + 2]), "r"(r[j + 3]) : "memory");
           }
-        } else if (there) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (c0 + j < w.rows) out[(size_t)(c0 + j) * p.ld_out] = from_f<TO>(v[j]);
         }
-        __syncwarp();
       }
-      tc_fence_before();
-      mbar_arrive(&acc_empty[b]);
     }
   }
   tc_fence_before();
+  if (p.splits > 1) {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (warp >= 2 && ok) {
+      const int4* part = (const int4*)sums + q * 32 + lane;
+      for (int i = 0; i < mine; i += 4) {
+        const int c = (split << shift) + i;
+        if (c >= rows) break;
+        int4 t = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+        for (int s = 0; s < p.splits; ++s) {
+          const int4 v = part[((s << shift) + i) * (BM / 4)];
+          t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+        }
+        finish(c, t.x);
+        if (c + 1 < rows) finish(c + 1, t.y);
+        if (c + 2 < rows) finish(c + 2, t.z);
+        if (c + 3 < rows) finish(c + 3, t.w);
+      }
+    }
+  }
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
@@ -348,23 +561,100 @@ bool make_map_i8(CUtensorMap* map, const void* ptr, long long rows, int K, long 
             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The packed tiles as rows of 128 bytes, copied as they are.
+bool make_map_tiles(CUtensorMap* map, const void* packed, long long tiles) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {QK, (cuuint64_t)tiles * BM};
+  cuuint64_t strides[1] = {QK};
+  cuuint32_t box[2] = {QK, BM};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)packed, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <bool GLU, typename TO, int RT, int STAGES>
-int launch_product(const CUtensorMap& map, const Int8Args& p, cudaStream_t st) {
-  constexpr int smem = STAGES * (W_TILE_BYTES + RT * QK) + 4 * RT * 4 + 1024 + 256;
+int launch_pair(const CUtensorMap& map_x, const CUtensorMap& map_w, const Int8Args& p, cudaStream_t st) {
+  constexpr int smem = STAGES * (W_TILE_BYTES + RT / 2 * QK) + 8 * (RT < 64 ? 32 : RT / 2) * 4 + 1024 + 256;
+  static_assert(smem <= 227 * 1024, "a CTA's shared memory");
   static PerDevice devices;
-  auto kernel = int8_product_kernel<GLU, TO, RT, STAGES>;
+  auto kernel = int8_pair_kernel<GLU, TO, RT, STAGES>;
   const int rc = qv_allow_smem(kernel, smem, devices);
   if (rc) return rc;
-  const long long items = (long long)p.row_tiles * ((p.N + BM - 1) / BM);
+  const long long items = (long long)p.row_tiles * ((p.N + 2 * BM - 1) / (2 * BM));
   if (items > 0x40000000LL) return QV_ERR_TOO_LARGE;
-  const int sms = sms_of_device();
-  return qv_launch(kernel, dim3((unsigned)(items < sms ? items : sms)), dim3(192), (size_t)smem, st, map, p);
+  const int pairs = sms_of_device() / 2;
+  return qv_launch_cluster(kernel, dim3(2 * (unsigned)(items < pairs ? items : pairs)), dim3(PAIR_THREADS), (size_t)smem, st, dim3(2, 1, 1), map_x, map_w, p);
 }
 
 template <int RT, int STAGES>
-int launch_product_as(const CUtensorMap& map, const Int8Args& p, bool glu, int out_dt, cudaStream_t st) {
-  if (glu) return out_dt == QV_DT_BF16 ? launch_product<true, bf16, RT, STAGES>(map, p, st) : launch_product<true, float, RT, STAGES>(map, p, st);
-  return out_dt == QV_DT_BF16 ? launch_product<false, bf16, RT, STAGES>(map, p, st) : launch_product<false, float, RT, STAGES>(map, p, st);
+int launch_pair_as(const CUtensorMap& map_x, const CUtensorMap& map_w, const Int8Args& p, bool glu, int out_dt, cudaStream_t st) {
+  if (glu) return out_dt == QV_DT_BF16 ? launch_pair<true, bf16, RT, STAGES>(map_x, map_w, p, st) : launch_pair<true, float, RT, STAGES>(map_x, map_w, p, st);
+  return out_dt == QV_DT_BF16 ? launch_pair<false, bf16, RT, STAGES>(map_x, map_w, p, st) : launch_pair<false, float, RT, STAGES>(map_x, map_w, p, st);
+}
+
+// CTAs that share a block of channels (1, 2 or 4), of at least 4 k blocks each: as many as the SMs hold at once, and up to 64 rows, whose sums
+// are cheap to hand over, a third more.  us with 1 / 2 / 4 / 8: 4096 x 14336, 1 row 22.1 / 14.0 / 12.9 / 12.6, 64 rows 30.6 / 23.7 / 17.5 / 21.1;
+// 2048 x 8192, 8 rows 14.0 / 9.8 / 7.4 / 10.7; 6144 x 4096 (48 blocks), 8 rows 9.2 / 8.4 / 8.1 / 9.7, 64 rows 12.7 / 12.1 / 11.0 / 15.5, 77 rows
+// 15.9 / 16.2 / 19.3; 28672 x 4096, 8 rows 22.4 / 25.5 / 26.5.
+int few_splits(int blocks, int rows, int KT, int sms) {
+  int splits = 1;
+  const int most = rows <= 64 ? sms + sms / 3 : sms;
+  while (splits < 4 && blocks * splits * 2 <= most && KT >= splits * 8) splits *= 2;
+#ifdef INT8_PROBE
+  if (getenv("QF_S")) return atoi(getenv("QF_S"));
+#endif
+  return splits;
+}
+
+// Whether the kernel for few rows takes a dense product: up to 64 rows, and up to 128 where four CTAs a block of channels find room (128 rows, 4096 x
+// 14336: 24.0 us against the pairs' 32.0; 77 rows, 6144 x 4096, where they do not: 16.1 against 12.8).
+bool few_rows(int rows, int N, int sms) { return rows <= 64 || (rows <= 128 && (N + BM - 1) / BM * 4 <= sms); }
+
+// Rows of the pairs' tiles, a multiple of 32: of the widths that need the least time, rounds of items times that of an item, the largest.  A k
+// block takes a pair 187 ns up to 64 rows, 235 at 128, 303 at 192 and 387 at 256 (2,048 rows, 28672 x 4096): what the SMs take in.
+int tile_rows_of(int rows, int N, int pairs) {
+  long long best = 0;
+  int width = 32;
+  for (int bn = 32; bn <= 256; bn += 32) {
+    const long long items = (long long)((rows + bn - 1) / bn) * ((N + 2 * BM - 1) / (2 * BM));
+    const long long cost = (items + pairs - 1) / pairs * ((bn < 64 ? 64 : bn) + 116);
+    if (bn == 32 || cost <= best) { best = cost; width = bn; }
+  }
+  return width;
+}
+
+template <bool GLU, typename TO, int BN, int STAGES>
+int launch_few(const CUtensorMap& map, Int8Args p, int blocks, int tiles, cudaStream_t st) {
+  auto kernel = int8_few_kernel<GLU, TO, BN, STAGES>;
+  p.mine_shift = 2;
+  while ((p.splits << p.mine_shift) < BN) ++p.mine_shift;
+  const int columns = p.splits > 1 ? p.splits << p.mine_shift : 0;
+  const size_t smem = STAGES * (W_TILE_BYTES + BN * QK) + 1024 + 256 + (size_t)columns * BM * 4;
+  constexpr size_t most = STAGES * (W_TILE_BYTES + BN * QK) + 1024 + 256 + (size_t)(BN < 32 ? 32 : BN) * BM * 4;
+  static_assert(most <= 227 * 1024, "a CTA's shared memory");
+  static PerDevice devices;
+  const int rc = qv_allow_smem(kernel, most, devices);
+  if (rc) return rc;
+  return qv_launch_cluster(kernel, dim3(blocks, tiles, p.splits), dim3(192), smem, st, dim3(1, 1, p.splits), map, p);
+}
+
+template <int BN, int DEEP, int SHALLOW>
+int launch_few_as(const CUtensorMap& map, Int8Args p, bool glu, int out_dt, cudaStream_t st) {
+  const int blocks = (p.N + BM - 1) / BM, KT = (p.K + QK - 1) / QK, tiles = (p.rows + BN - 1) / BN, sms = sms_of_device();
+  if (tiles > 65535) return QV_ERR_TOO_LARGE;
+  const int splits = few_splits(blocks * tiles, p.rows, KT, sms);
+  p.kb_per_split = (KT + splits - 1) / splits;
+  p.splits = (KT + p.kb_per_split - 1) / p.kb_per_split;       // none without k blocks
+  const bool one_wave = (long long)blocks * tiles * p.splits <= sms;
+#define FEW(GLU, TO) return one_wave ? launch_few<GLU, TO, BN, DEEP>(map, p, blocks, tiles, st) : launch_few<GLU, TO, BN, SHALLOW>(map, p, blocks, tiles, st)
+  if (glu) {
+    if (out_dt == QV_DT_BF16) FEW(true, bf16);
+    FEW(true, float);
+  }
+  if (out_dt == QV_DT_BF16) FEW(false, bf16);
+  FEW(false, float);
+#undef FEW
 }
 
 #define INT8_MAX_K 131071             // 128 * 128 * K stays below 2^31
@@ -424,22 +714,39 @@ extern "C" int qv_gemm_int8(void* out, long long ld_out, int out_dt, const int8_
   p.out = out; p.x_scale = x_scale; p.w = (const uint8_t*)w; p.w_scale = w_scale; p.tiles = tiles; p.err = err; p.ld_out = ld_out;
   p.rows = rows; p.N = N; p.K = K; p.experts = E;
   p.glu = {glu ? act : 0, limit, slope};
+  cudaStream_t st = (cudaStream_t)stream;
+  CUtensorMap map, map_w;
+  int few = few_rows(rows, N, sms_of_device());
+#ifdef INT8_PROBE
+  if (getenv("QF_T")) few = rows <= atoi(getenv("QF_T"));
+#endif
+  if (!tiles && few) {
+    const int bn = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    if (!make_map_i8(&map, x, rows, K, ld_x, bn)) return QV_ERR_UNSUPPORTED;
+    if (bn == 16) return launch_few_as<16, 10, 5>(map, p, glu, out_dt, st);
+    if (bn == 32) return launch_few_as<32, 9, 4>(map, p, glu, out_dt, st);
+    if (bn == 64) return launch_few_as<64, 7, 3>(map, p, glu, out_dt, st);
+    return launch_few_as<128, 4, 3>(map, p, glu, out_dt, st);
+  }
   int rt;
   if (tiles) {
     if (max_tiles <= 0) return 0;
-    rt = tile_rows; p.box = 32; p.bn = tile_rows; p.row_tiles = max_tiles;
+    rt = tile_rows; p.bn = tile_rows; p.row_tiles = max_tiles; p.box = 16;
   } else {
-    p.bn = rows < 256 ? (rows + 15) & ~15 : 256;
+    p.bn = tile_rows_of(rows, N, sms_of_device() / 2);
+#ifdef INT8_PROBE
+    if (getenv("QF_BN")) p.bn = atoi(getenv("QF_BN"));
+#endif
     rt = p.bn <= 32 ? 32 : p.bn <= 64 ? 64 : p.bn <= 128 ? 128 : 256;
-    p.box = p.bn; p.row_tiles = (rows + p.bn - 1) / p.bn;
+    p.box = p.bn / 2; p.row_tiles = (rows + p.bn - 1) / p.bn;
   }
-  CUtensorMap map;
-  if (!make_map_i8(&map, x, rows, K, ld_x, p.box)) return QV_ERR_UNSUPPORTED;
-  cudaStream_t st = (cudaStream_t)stream;
-  if (rt == 32) return launch_product_as<32, 10>(map, p, glu, out_dt, st);
-  if (rt == 64) return launch_product_as<64, 8>(map, p, glu, out_dt, st);
-  if (rt == 128) return launch_product_as<128, 6>(map, p, glu, out_dt, st);
-  if (rt == 256) return launch_product_as<256, 4>(map, p, glu, out_dt, st);
+  const long long w_tiles = (long long)E * ((N + BM - 1) / BM) * ((K + QK - 1) / QK);
+  if (w_tiles * BM > 0x7fffffffLL) return QV_ERR_TOO_LARGE;     // rows of the tensor map are counted in 31 bits
+  if (!make_map_i8(&map, x, rows, K, ld_x, p.box) || !make_map_tiles(&map_w, w, w_tiles)) return QV_ERR_UNSUPPORTED;
+  if (rt == 32) return launch_pair_as<32, 11>(map, map_w, p, glu, out_dt, st);
+  if (rt == 64) return launch_pair_as<64, 10>(map, map_w, p, glu, out_dt, st);
+  if (rt == 128) return launch_pair_as<128, 8>(map, map_w, p, glu, out_dt, st);
+  if (rt == 256) return launch_pair_as<256, 6>(map, map_w, p, glu, out_dt, st);
   return QV_ERR_UNSUPPORTED;
 }
 
