@@ -450,27 +450,41 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
 }
 
 // ---------------------------------------------------------------- rows in 8 bits
-// One read and one write of the row are all it cannot do without, so a row stays in registers between its maximum and its rounding: VECS
-// pieces of 16 bytes a thread, all asked for at once.  A row has a block of its own, whose size goes by the row's length; rows longer than
-// VECS pieces of 1,024 threads are read twice (LONG).  ALIGNED: pieces lie on 16 bytes; else their entries are read one by one.
+// One read and one write of the row are all it cannot do without, so a row stays in registers, as stored, between its maximum and its
+// rounding: VECS pieces of 16 bytes a thread, all asked for at once.  A row has a warp (no barrier between its two halves, so that the SM's
+// other rows go on: many short rows) or a block; rows longer than VECS pieces of 1,024 threads are read twice (LONG).  ALIGNED: pieces lie
+// on 16 bytes; else their entries are read one by one.
 template <typename T> struct Piece { static constexpr int N = 16 / (int)sizeof(T); };
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void load_piece(float (&f)[Piece<T>::N], const T* x, int k, int K) {
+template <typename T, bool ALIGNED> __device__ __forceinline__ uint4 load_piece(const T* x, int k, int K) {
   constexpr int N = Piece<T>::N;
-  if (ALIGNED && k + N <= K) {
-    const uint4 v = *(const uint4*)(x + k);
-    const T* e = (const T*)&v;
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (ALIGNED && k + N <= K) return *(const uint4*)(x + k);
+  T* e = (T*)&v;
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = to_f(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = k + i < K ? to_f(x[k + i]) : 0.f;
-  }
+  for (int i = 0; i < N; ++i)
+    if (k + i < K) e[i] = x[k + i];
+  return v;
 }
-template <int N>
-__device__ __forceinline__ void store_piece(int8_t* q, const float (&f)[N], const Int8Scale& s, int k, int K) {
+// The largest magnitude so far, of bfloat16 a pair of them (their bits are ordered as float32's are).
+__device__ __forceinline__ uint32_t larger(uint32_t top, const uint4& v, const float*) {
+  constexpr uint32_t M = 0x7fffffffu;
+  return max(max(top, max(v.x & M, v.y & M)), max(v.z & M, v.w & M));
+}
+__device__ __forceinline__ uint32_t larger(uint32_t top, const uint4& v, const bf16*) {
+  constexpr uint32_t M = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(top, __vmaxu2(v.x & M, v.y & M)), __vmaxu2(v.z & M, v.w & M));
+}
+__device__ __forceinline__ uint32_t top_bits(uint32_t top, const float*) { return top; }
+__device__ __forceinline__ uint32_t top_bits(uint32_t top, const bf16*) { return max(top << 16, top & 0xffff0000u); }
+
+template <typename T> __device__ __forceinline__ void store_piece(int8_t* q, const uint4& v, const Int8Scale& s, int k, int K) {
+  constexpr int N = Piece<T>::N;
+  float f[N];
+  const T* e = (const T*)&v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = to_f(e[i]);
   uint32_t w[N / 4];
-  int8_pack<N>(f, s, w);
+  int8_pack<sizeof(T) == 2, N>(f, s, w);
   if (k + N <= K) {
     if (N == 8) *(uint2*)(q + k) = make_uint2(w[0], w[N / 4 - 1]);
     else *(uint32_t*)(q + k) = w[0];
@@ -481,46 +495,42 @@ __device__ __forceinline__ void store_piece(int8_t* q, const float (&f)[N], cons
   }
 }
 
-template <typename T, int VECS, bool ALIGNED, bool LONG>
-__global__ void __launch_bounds__(1024) quantize_rows_kernel(int8_t* __restrict__ q, long long ld_q, float* __restrict__ scale, const T* __restrict__ x,
-                                                             long long ld_x, const int* __restrict__ row_idx, int rows_in, int K) {
+#define QUANTIZE_WARPS 4              // rows of a block whose rows have a warp each
+template <typename T, int VECS, bool WARP, bool ALIGNED, bool LONG>
+__global__ void __launch_bounds__(WARP ? 32 * QUANTIZE_WARPS : 1024) quantize_rows_kernel(int8_t* __restrict__ q, long long ld_q, float* __restrict__ scale,
+                                                                                         const T* __restrict__ x, long long ld_x,
+                                                                                         const int* __restrict__ row_idx, int rows_in, int rows, int K) {
   constexpr int N = Piece<T>::N;
   __shared__ uint32_t red[32];
   pdl_wait();
   pdl_launch_dependents();
-  const int r = blockIdx.x, step = blockDim.x * N;
+  const int r = WARP ? blockIdx.x * QUANTIZE_WARPS + (threadIdx.x >> 5) : blockIdx.x;
+  const int at = (WARP ? threadIdx.x & 31 : threadIdx.x) * N, step = (WARP ? 32 : blockDim.x) * N;
+  if (WARP && r >= rows) return;
   const int src = row_idx ? row_idx[r] : r;
   const bool there = (unsigned)src < (unsigned)rows_in;      // an index outside the rows: a row of zeros
   const T* xr = x + (size_t)(there ? src : 0) * ld_x;
   const int n = there ? K : 0;
   int8_t* o = q + (size_t)r * ld_q;
-  float f[VECS][N];
+  uint4 v[VECS];
   uint32_t top = 0;
   if (LONG) {
-    for (int k = threadIdx.x * N; k < n; k += step) {
-      load_piece<T, ALIGNED>(f[0], xr, k, n);
-#pragma unroll
-      for (int i = 0; i < N; ++i) top = max(top, int8_bits(f[0][i]));
-    }
+    for (int k = at; k < n; k += step) top = larger(top, load_piece<T, ALIGNED>(xr, k, n), xr);
   } else {
 #pragma unroll
-    for (int v = 0; v < VECS; ++v) load_piece<T, ALIGNED>(f[v], xr, threadIdx.x * N + v * step, n);
+    for (int i = 0; i < VECS; ++i) v[i] = load_piece<T, ALIGNED>(xr, at + i * step, n);
 #pragma unroll
-    for (int v = 0; v < VECS; ++v)
-#pragma unroll
-      for (int i = 0; i < N; ++i) top = max(top, int8_bits(f[v][i]));
+    for (int i = 0; i < VECS; ++i) top = larger(top, v[i], xr);
   }
-  const Int8Scale s = int8_scale(int8_block_top(top, red));
-  if (threadIdx.x == 0) scale[r] = s.scale;
+  top = top_bits(top, xr);
+  const Int8Scale s = int8_scale(WARP ? __uint_as_float(__reduce_max_sync(0xffffffffu, top)) : int8_block_top(top, red));
+  if (at == 0) scale[r] = s.scale;
   if (LONG) {
-    for (int k = threadIdx.x * N; k < K; k += step) {
-      load_piece<T, ALIGNED>(f[0], xr, k, n);
-      store_piece<N>(o, f[0], s, k, K);
-    }
+    for (int k = at; k < K; k += step) store_piece<T>(o, load_piece<T, ALIGNED>(xr, k, n), s, k, K);
   } else {
 #pragma unroll
-    for (int v = 0; v < VECS; ++v)
-      if (threadIdx.x * N + v * step < K) store_piece<N>(o, f[v], s, threadIdx.x * N + v * step, K);
+    for (int i = 0; i < VECS; ++i)
+      if (at + i * step < K) store_piece<T>(o, v[i], s, at + i * step, K);
   }
 }
 
@@ -680,18 +690,20 @@ extern "C" int qv_quantize_rows(int8_t* q, long long ld_q, float* scale, const v
   if (T <= 0) return 0;
   if (K <= 0 || ld_q < K || ((uintptr_t)q & 15) || (ld_q & 15) || ld_x < K || (!row_idx && rows_in < T)) return QV_ERR_UNSUPPORTED;
   cudaStream_t st = (cudaStream_t)stream;
-#define QUANTIZE(VECS, ALIGNED, LONG, THREADS)                                                                                                          \
-  return qv_launch(quantize_rows_kernel<TX, VECS, ALIGNED, LONG>, dim3(T), dim3(THREADS), 0, st, q, ld_q, scale, (const TX*)x, ld_x, row_idx, rows_in, K)
-#define QUANTIZE_AS(ALIGNED)                                                             \
-  do {                                                                                   \
-    if (pieces > 4096) QUANTIZE(1, ALIGNED, true, 1024);                                 \
-    if (few && pieces <= 1024) QUANTIZE(1, ALIGNED, false, (pieces + 31) / 32 * 32);     \
-    if (pieces <= 512) QUANTIZE(2, ALIGNED, false, (pieces + 63) / 64 * 32);             \
-    QUANTIZE(4, ALIGNED, false, (pieces + 127) / 128 * 32);                              \
+#define QUANTIZE(VECS, WARP, ALIGNED, LONG, THREADS)                                                                                                     \
+  return qv_launch(quantize_rows_kernel<TX, VECS, WARP, ALIGNED, LONG>, dim3(WARP ? (T + QUANTIZE_WARPS - 1) / QUANTIZE_WARPS : T), dim3(THREADS), 0, st, q, \
+                   ld_q, scale, (const TX*)x, ld_x, row_idx, rows_in, T, K)
+#define QUANTIZE_AS(ALIGNED)                                                                   \
+  do {                                                                                         \
+    if (pieces > 4096) QUANTIZE(1, false, ALIGNED, true, 1024);                                \
+    if (few && pieces <= 1024) QUANTIZE(1, false, ALIGNED, false, (pieces + 31) / 32 * 32);    \
+    if (pieces <= 128) QUANTIZE(4, true, ALIGNED, false, 32 * QUANTIZE_WARPS);                 \
+    if (pieces <= 256) QUANTIZE(8, true, ALIGNED, false, 32 * QUANTIZE_WARPS);                 \
+    QUANTIZE(4, false, ALIGNED, false, (pieces + 127) / 128 * 32);                             \
   } while (0)
   QV_DISPATCH_DT(x_dt, TX, {
     const int pieces = (K + Piece<TX>::N - 1) / Piece<TX>::N;
-    const bool few = T <= 2 * sms_of_device();
+    const bool few = T <= 2 * sms_of_device();                  // blocks of as many threads as a row has pieces find room at once
     if (((uintptr_t)x & 15) == 0 && (ld_x * sizeof(TX)) % 16 == 0) QUANTIZE_AS(true);
     QUANTIZE_AS(false);
   });

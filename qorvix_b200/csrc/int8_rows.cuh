@@ -1,9 +1,13 @@
 // Rows in 8-bit integers: q_k = round(127 x_k / top), ties to the even one, and the scale top / 127, with top = max_k |x_k|.
 //   top 0:           scale 0, q 0
 //   top not finite:  scale NaN, q 0 (every product with the row is NaN, as it is in floating arithmetic)
-// The quotient is the exact one: q does not depend on how a kernel forms it.  In float32 it is off by at most 2^-23 of itself, under
-// 2e-5; only where it comes out nearer than 1e-4 to the border between two numbers is it decided in float64, where 127 |x| and
-// (n + 1/2) top are both exact (31 and 32 bits).  What is rounded has then lost half a step of 1/127 of the row's largest entry, no more.
+// The quotient is the exact one: q does not depend on how a kernel forms it.  v = x * (127 / top) in float32 is off by at most 2^-22 of itself.
+//   bfloat16 entries: 127 x / top = a / b with whole a up to 127 * 255 and b up to 255, times a power of two; where it is not a half-integer it
+//     differs from every one by 2^-17 of itself or more.  So v rounded to 20 bits is a half-integer just where the quotient is one, and lies
+//     on the quotient's side of it elsewhere.  No entry needs a second look (one in 200 lies on a border; looking at those cost half
+//     the time of a pass).
+//   float32 entries: where v comes out nearer than 1e-4 to a border, the exact products decide.
+// What is rounded has then lost half a step of 1/127 of the row's largest entry, no more.
 #pragma once
 #include "common.cuh"
 
@@ -24,38 +28,77 @@ __device__ __forceinline__ Int8Scale int8_scale(float top) {
   return s;
 }
 
-// The row's entry x (times s.pre), whose quotient v is next to a border.
-__device__ __noinline__ float int8_border(float x, float v, float top) {
-  const float lo = floorf(fabsf(v));
-  const double a = 127.0 * (double)fabsf(x), h = ((double)lo + 0.5) * (double)top;
-  const float r = a > h || (a == h && ((int)lo & 1)) ? lo + 1.f : lo;
-  return copysignf(r, x);
+// The row's entry x (times s.pre), whose quotient lies next to the border on the side d of the number r that t = r + 1.5 2^23 holds: whether it
+// goes to r or to the next number on that side, as t.  With m = r +- 1/2, 127 x and m top differ by less than 2^-13 of themselves; with p =
+// m top rounded, both 127 x - p and what p was rounded by come out of a multiply-add exactly, so their order is that of the two products.
+__device__ __forceinline__ float int8_border(float x, float t, float d, float top) {
+  const float m = (t - 12582912.f) + copysignf(0.5f, d);
+  const float p = m * top, off = fmaf(m, top, -p), a = fmaf(127.f, x, -p);
+  const bool beyond = d > 0.f ? a > off : a < off;
+  return beyond || (a == off && (__float_as_uint(t) & 1u)) ? t + copysignf(1.f, d) : t;
 }
 
-// Entries of a row as bytes, N of them (a multiple of 4) packed in words.  t = v + 1.5 2^23 holds round(v) in its low bits; v - round(v) says
-// how near the border lies, and the whole group is looked at once.
-template <int N>
-__device__ __forceinline__ void int8_pack(const float (&x)[N], const Int8Scale& s, uint32_t (&out)[N / 4]) {
+// Two operations an instruction, each half rounded as the one it stands for.
+union FloatPair { float2 f; unsigned long long u; };
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
+  FloatPair x{a}, y{b}, z{c}, r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(x.u), "l"(y.u), "l"(z.u));
+  return r.f;
+}
+__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
+  FloatPair x{a}, y{b}, r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(x.u), "l"(y.u));
+  return r.f;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+  FloatPair x{a}, y{b}, r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(x.u), "l"(y.u));
+  return r.f;
+}
+
+// Entries of a row as bytes, N of them (a multiple of 4) packed in words; BF16: they are bfloat16 numbers.  t = v + 1.5 2^23 holds round(v) in
+// its low bits.  The instructions of this function are what bounds passes over many rows.
+template <bool BF16, int N>
+__device__ __forceinline__ void int8_pack(float (&x)[N], const Int8Scale& s, uint32_t (&out)[N / 4]) {
   constexpr float MAGIC = 12582912.f;
-  float t[N], far = 0.f;
+  if (!s.live) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float xi = x[i] * s.pre;
-    t[i] = fmaf(xi, s.inv, MAGIC);
-    far = fmaxf(far, fabsf(fmaf(xi, s.inv, MAGIC - t[i])));
+    for (int i = 0; i < N / 4; ++i) out[i] = 0u;
+    return;
   }
-  if (far > 0.4999f) {
+  if (s.pre != 1.f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= s.pre;
+  }
+  float t[N], far = 0.f;
+  const float2 inv = make_float2(s.inv, s.inv), magic = make_float2(MAGIC, MAGIC), minus = make_float2(-1.f, -1.f), split = make_float2(17.f, 17.f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    float2 v = make_float2(x[i], x[i + 1]), r;
+    if (BF16) {
+      v = mul_pair(v, inv);
+      const float2 p = mul_pair(v, split);           // p - (p - v): v rounded to 20 bits
+      r = add_pair(fma_pair(fma_pair(v, minus, p), minus, p), magic);
+    } else {
+      r = fma_pair(v, inv, magic);
+      const float2 d = fma_pair(v, inv, fma_pair(r, minus, magic));
+      far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+    }
+    t[i] = r.x;
+    t[i + 1] = r.y;
+  }
+  if (!BF16 && far > 0.4999f) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float xi = x[i] * s.pre, v = xi * s.inv;
-      if (fabsf(fmaf(xi, s.inv, MAGIC - t[i])) > 0.4999f) t[i] = MAGIC + int8_border(xi, v, s.top);
+      const float d = fmaf(x[i], s.inv, MAGIC - t[i]);
+      if (fabsf(d) > 0.4999f) t[i] = int8_border(x[i], t[i], d, s.top);
     }
   }
 #pragma unroll
   for (int i = 0; i < N; i += 4) {
     const uint32_t lo = __byte_perm(__float_as_uint(t[i]), __float_as_uint(t[i + 1]), 0x0040);
     const uint32_t hi = __byte_perm(__float_as_uint(t[i + 2]), __float_as_uint(t[i + 3]), 0x0040);
-    out[i / 4] = s.live ? __byte_perm(lo, hi, 0x5410) : 0u;
+    out[i / 4] = __byte_perm(lo, hi, 0x5410);
   }
 }
 

@@ -182,9 +182,9 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
   if (threadIdx.x == 0) a.out_scale[t] = s.scale;
   int8_t* o = (int8_t*)a.out + (size_t)t * a.ld_out;
   auto put = [&](int i, float4 v) {
-    const float f[4] = {v.x, v.y, v.z, v.w};
+    float f[4] = {v.x, v.y, v.z, v.w};
     uint32_t w[1];
-    int8_pack<4>(f, s, w);
+    int8_pack<true, 4>(f, s, w);
     if (i + 4 <= d) { *(uint32_t*)(o + i) = w[0]; return; }
     for (int k = 0; i + k < d; ++k) o[i + k] = (int8_t)(w[0] >> (8 * k));
   };

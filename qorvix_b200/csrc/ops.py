@@ -1792,7 +1792,7 @@ class Int8Weight:
     """A matrix [N, K] of 8-bit integers with a scale a row, or `experts` of them (0: one), laid out for the products (pack_int8)."""
     __slots__ = ("packed", "scale", "n", "k", "experts")
 
-    def __init__(self, packed, scale, n: int, k: int, experts: int):
+    def __init__(self, packed, scale, n: int, k: int, experts: int = 0):
         self.packed, self.scale, self.n, self.k, self.experts = packed, scale, n, k, experts
 
     @property
@@ -1800,13 +1800,27 @@ class Int8Weight:
         return self.packed.device
 
 
-def _on_current(*tensors) -> None:
-    """All on the device that launches go to."""
-    _need_cuda(*tensors)
+def _on_current(*tensors) -> int:
+    """The device that launches go to, on which all must live."""
+    _need_cuda(tensors[0])
     dev = _get_device() if _get_device is not None else torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
+            _need_cuda(t)
             raise KernelError(f"kernel operands must live on the current CUDA device ({dev}), not on {t.device}")
+    return dev
+
+
+_DT = {torch.float32: F32, torch.bfloat16: BF16}
+_err_words = {}
+
+
+def _err_word(dev: int) -> int:
+    """The address of the device's error word."""
+    p = _err_words.get(dev)
+    if p is None:
+        p = _err_words[dev] = _tc_buffers(torch.device("cuda", dev))["err"].data_ptr()
+    return p
 
 
 def int8_rows(tokens: int, k: int, device) -> Int8Rows:
@@ -1817,38 +1831,35 @@ def int8_rows(tokens: int, k: int, device) -> Int8Rows:
 
 def _int8_rows_checked(rows: Int8Rows) -> Int8Rows:
     v, s = rows.values, rows.scale
-    if v.dtype != torch.int8 or v.dim() != 2 or s.dtype != torch.float32 or s.shape != v.shape[:1] or not s.is_contiguous():
+    shape, strides = v.shape, v.stride()
+    if v.dtype != torch.int8 or len(shape) != 2 or s.dtype != torch.float32 or s.shape != shape[:1] or not s.is_contiguous() or s.device != v.device:
         raise KernelError("8-bit rows are int8 [T, K] with a contiguous float32 scale [T]")
-    if v.stride(1) != 1 or (v.shape[0] > 1 and (v.stride(0) % 16 or v.stride(0) < v.shape[1])) or v.data_ptr() % 16:
+    if strides[1] != 1 or (shape[0] > 1 and (strides[0] % 16 or strides[0] < shape[1])) or v.data_ptr() % 16:
         raise KernelError("8-bit rows must start on 16 bytes (int8_rows makes such room)")
     return rows
-
-
-def _ld(t) -> int:
-    """The row stride of a matrix; of a single row, whose stride says nothing, its width."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
 def quantize_rows(rows: Int8Rows, x, row_idx=None) -> None:
     """rows[r] = x[r], or x[row_idx[r]], in 8 bits: values = round(127 x / max|x|) (the exact quotient; ties to the even one), scale =
     max|x| / 127.  x float32 or bfloat16, rows may be strided.  A row of zeros has scale 0; one that holds an infinity or a NaN has scale
     NaN; an index outside x's rows gives a row of zeros."""
-    _int8_rows_checked(rows)
-    _on_current(rows.values, rows.scale, x, row_idx)
-    T, K = rows.values.shape
-    if x.dim() != 2 or x.shape[1] != K or (K > 1 and x.stride(1) != 1):
-        raise KernelError(f"rows of {K} entries wanted, whole in memory, not {tuple(x.shape)} with strides {x.stride()}")
+    v = _int8_rows_checked(rows).values
+    T, K = v.shape
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 2 or shape[1] != K or (K > 1 and strides[1] != 1):
+        raise KernelError(f"rows of {K} entries wanted, whole in memory, not {tuple(shape)} with strides {strides}")
     if row_idx is None:
-        if x.shape[0] != T:
-            raise KernelError(f"{x.shape[0]} rows do not fill {T}")
+        if shape[0] != T:
+            raise KernelError(f"{shape[0]} rows do not fill {T}")
     else:
         _i32(row_idx, "row_idx")
         if row_idx.numel() != T:
             raise KernelError(f"{row_idx.numel()} row indices do not fill {T} rows")
     if T == 0:
         return
-    rc = _lib("gemm_int8").qv_quantize_rows(_ptr(rows.values), _ld16(rows.values), _ptr(rows.scale), _ptr(x), _ld(x), dt_code(x.dtype), _ptr(row_idx),
-                                            x.shape[0], T, K, _stream())
+    _on_current(v, x, row_idx)
+    rc = _lib("gemm_int8").qv_quantize_rows(v.data_ptr(), _ld16(v), rows.scale.data_ptr(), x.data_ptr(), strides[0] if shape[0] > 1 else K, dt_code(x.dtype),
+                                            _ptr(row_idx), shape[0], T, K, _stream())
     _check(rc, "quantize_rows")
 
 
@@ -1883,35 +1894,37 @@ def quantize_weight(w) -> Int8Weight:
 
 
 def _int8_product(out, x, weight: Int8Weight, act: int, limit: float, slope: float, what: str) -> None:
+    rows8 = isinstance(x, Int8Rows)
+    v = _int8_rows_checked(x).values if rows8 else x
     n = weight.n if act < 0 else weight.n // 2
+    shape, strides = v.shape, v.stride()
+    T = shape[0]
     if weight.experts:
         raise KernelError(f"{what} takes one matrix; experts' matrices go to moe_experts_int8")
-    if act >= 0 and (weight.n % 32 or act not in (GLU_SILU, GLU_GELU_TANH, GLU_CLAMPED)):
+    if act >= 0 and (weight.n % 32 or act > 2):
         raise KernelError(f"{what}: gate and up rows alternate in groups of 16, and act is GLU_SILU, GLU_GELU_TANH or GLU_CLAMPED")
-    T, K = x.shape
-    if K != weight.k or out.dim() != 2 or out.shape[0] != T or out.shape[1] != n or (n > 1 and out.stride(1) != 1):
-        raise KernelError(f"{what}: rows {tuple(x.shape)} and a matrix of {weight.n} x {weight.k} do not give {tuple(out.shape)}")
-    if T > 1 and out.stride(0) < n:
-        raise KernelError(f"{what}: the output's rows overlap")
+    if len(shape) != 2 or shape[1] != weight.k or out.shape != (T, n):
+        raise KernelError(f"{what}: rows {tuple(shape)} and a matrix of {weight.n} x {weight.k} do not give {tuple(out.shape)}")
+    out_strides = out.stride()
+    ld_out = out_strides[0] if T > 1 else n
+    if (n > 1 and out_strides[1] != 1) or ld_out < n or (weight.k > 1 and strides[1] != 1):
+        raise KernelError(f"{what}: rows must be whole in memory and must not overlap, not strides {strides} and {out_strides}")
     if T == 0:
         return
-    lib = _lib("gemm_int8")
-    err = _ptr(_tc_buffers(out.device)["err"])
-    if isinstance(x, Int8Rows):
-        _int8_rows_checked(x)
-        _on_current(out, x.values, x.scale, weight.packed)
-        rc = lib.qv_gemm_int8(_ptr(out), _ld(out), dt_code(out.dtype), _ptr(x.values), _ld16(x.values), _ptr(x.scale), _ptr(weight.packed), _ptr(weight.scale),
-                              T, weight.n, K, 1, None, 0, 0, act, float(limit), float(slope), err, _stream())
+    dev = _on_current(out, v, weight.packed)
+    lib, K, dt = _lib("gemm_int8"), weight.k, _DT.get(out.dtype)
+    dt = dt_code(out.dtype) if dt is None else dt
+    ld = strides[0] if T > 1 else -(-K // 16) * 16
+    if rows8:
+        rc = lib.qv_gemm_int8(out.data_ptr(), ld_out, dt, v.data_ptr(), ld, x.scale.data_ptr(), weight.packed.data_ptr(), weight.scale.data_ptr(),
+                              T, weight.n, K, 1, None, 0, 0, act, limit, slope, _err_word(dev), _stream())
         _check(rc, what)
         return
-    _on_current(out, x, weight.packed)
-    if K > 1 and x.stride(1) != 1:
-        raise KernelError(f"{what}: rows must be whole in memory, not strides {x.stride()}")
-    ld = -(-K // 16) * 16
-    room = torch.empty(T * (ld + 4), device=x.device, dtype=torch.int8)        # the rows in 8 bits, then their scales
+    ldq = -(-K // 16) * 16
+    room = x.new_empty(T * (ldq + 4), dtype=torch.int8)                        # the rows in 8 bits, then their scales
     q = room.data_ptr()
-    rc = lib.qv_linear_int8(_ptr(out), _ld(out), dt_code(out.dtype), _ptr(x), _ld(x), dt_code(x.dtype), q, ld, q + T * ld, _ptr(weight.packed),
-                            _ptr(weight.scale), T, weight.n, K, act, float(limit), float(slope), err, _stream())
+    rc = lib.qv_linear_int8(out.data_ptr(), ld_out, dt, x.data_ptr(), ld, dt_code(x.dtype), q, ldq, q + T * ldq, weight.packed.data_ptr(),
+                            weight.scale.data_ptr(), T, weight.n, K, act, limit, slope, _err_word(dev), _stream())
     _check(rc, what)
     add_launches(1)
 
@@ -1939,23 +1952,22 @@ def moe_experts_int8(up, out, rows: Int8Rows, weight: Int8Weight, tiles, act: in
     gemm_int8_glu), False: out [R, N] the products themselves; float32 or bfloat16.  tiles: moe_group's table, made for tiles of `tile_rows`
     rows (moe_int8_tile_rows).  Rows that no tile lists are left as they were."""
     n = weight.n // 2 if up else weight.n
-    _int8_rows_checked(rows)
-    _on_current(out, rows.values, rows.scale, weight.packed, tiles)
+    v = _int8_rows_checked(rows).values
+    R, K = v.shape
     _i32(tiles, "tiles")
-    R, K = rows.shape
-    if not weight.experts or tile_rows not in INT8_TILE_ROWS:
-        raise KernelError("moe_experts_int8 takes experts' matrices and tiles of 32, 64, 128 or 256 rows")
+    if not weight.experts or tile_rows not in INT8_TILE_ROWS or tiles.numel() % 3:
+        raise KernelError("moe_experts_int8 takes experts' matrices and a table, of three numbers a tile, of tiles of 32, 64, 128 or 256 rows")
     if up and (weight.n % 32 or act not in (GLU_SILU, GLU_GELU_TANH, GLU_CLAMPED)):
         raise KernelError("moe_experts_int8: gate and up rows alternate in groups of 16, and act is GLU_SILU, GLU_GELU_TANH or GLU_CLAMPED")
-    if K != weight.k or tuple(out.shape) != (R, n) or (n > 1 and out.stride(1) != 1) or (R > 1 and out.stride(0) < n):
-        raise KernelError(f"moe_experts_int8: rows {tuple(rows.shape)} and matrices of {weight.n} x {weight.k} do not give {tuple(out.shape)}")
-    if tiles.numel() % 3:
-        raise KernelError("the tile table holds three numbers a tile")
+    if K != weight.k:
+        raise KernelError(f"moe_experts_int8: rows {tuple(v.shape)} do not go with matrices of {weight.n} x {weight.k}")
+    ld_out, out_dt = _rows_of(out, (R, n), "out")
     if R == 0 or tiles.numel() == 0:
         return
-    rc = _lib("gemm_int8").qv_gemm_int8(_ptr(out), _ld(out), dt_code(out.dtype), _ptr(rows.values), _ld16(rows.values), _ptr(rows.scale), _ptr(weight.packed),
-                                        _ptr(weight.scale), R, weight.n, K, weight.experts, _ptr(tiles), tiles.numel() // 3, tile_rows, int(act) if up else -1,
-                                        float(limit), float(slope), _ptr(_tc_buffers(out.device)["err"]), _stream())
+    dev = _on_current(out, v, weight.packed, tiles)
+    rc = _lib("gemm_int8").qv_gemm_int8(out.data_ptr(), ld_out, out_dt, v.data_ptr(), _ld16(v), rows.scale.data_ptr(), weight.packed.data_ptr(),
+                                        weight.scale.data_ptr(), R, weight.n, K, weight.experts, tiles.data_ptr(), tiles.numel() // 3, tile_rows,
+                                        int(act) if up else -1, limit, slope, _err_word(dev), _stream())
     _check(rc, "moe_experts_int8")
 
 
@@ -1967,34 +1979,52 @@ def norm_gate_add(residual, y=None, post_weight=None, post_eps: float = 0.0, gat
     float32 or bfloat16 (rows may be strided); the weights, gate_bias and scale float32 [d]; out None, float32, bfloat16 (rows may be strided)
     or Int8Rows (the bfloat16 rows in 8 bits, see quantize_rows)."""
     rows8 = isinstance(out, Int8Rows)
-    if rows8:
-        _int8_rows_checked(out)
-    o = out.values if rows8 else out
-    _on_current(residual, y, post_weight, gate, gate_bias, scale, next_weight, o, into)
-    T, d = residual.shape
+    o = _int8_rows_checked(out).values if rows8 else out
     into = residual if into is None else into
-    if residual.dtype != torch.float32 or not residual.is_contiguous() or into.dtype != torch.float32 or not into.is_contiguous() or into.shape != residual.shape:
+    shape = residual.shape
+    T, d = shape
+    dev = _on_current(residual, y, post_weight, gate, gate_bias, scale, next_weight, o, into)
+    if residual.dtype != torch.float32 or not residual.is_contiguous():
         raise KernelError("the residual stream is contiguous float32 [T, d]")
-    if into is not residual and into.data_ptr() != residual.data_ptr() and abs(into.data_ptr() - residual.data_ptr()) < residual.nbytes:
-        raise KernelError("the new residual stream lies partly over the old one")
-    for t, name in ((y, "y"), (gate, "gate"), (o, "out")):
-        if t is not None and (tuple(t.shape) != (T, d) or (d > 1 and t.stride(1) != 1)):
-            raise KernelError(f"{name} must be [{T}, {d}] with whole rows, not {tuple(t.shape)} with strides {t.stride()}")
-    for t, name in ((post_weight, "post_weight"), (gate_bias, "gate_bias"), (scale, "scale"), (next_weight, "next_weight")):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != d or not t.is_contiguous()):
-            raise KernelError(f"{name} must be contiguous float32 [{d}]")
-    if y is None and (post_weight is not None or gate is not None or scale is not None):
+    if into is not residual:
+        if into.dtype != torch.float32 or into.shape != shape or not into.is_contiguous():
+            raise KernelError("the new residual stream is contiguous float32 [T, d]")
+        apart = abs(into.data_ptr() - residual.data_ptr())
+        if 0 < apart < 4 * T * d:
+            raise KernelError("the new residual stream lies partly over the old one")
+    ld_y = ld_gate = ld_out = d
+    y_dt = gate_dt = out_kind = F32
+    if y is not None:
+        ld_y, y_dt = _rows_of(y, shape, "y")
+        if gate is not None:
+            ld_gate, gate_dt = _rows_of(gate, shape, "gate")
+    elif post_weight is not None or gate is not None or scale is not None:
         raise KernelError("a norm, a gate or a scale needs a y")
+    if rows8:
+        if o.shape != shape:
+            raise KernelError(f"out must be {tuple(shape)}, not {tuple(o.shape)}")
+        ld_out, out_kind = _ld16(o), 2
+    elif o is not None:
+        ld_out, out_kind = _rows_of(o, shape, "out")
+    for t in (post_weight, gate_bias, scale, next_weight):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != d or not t.is_contiguous()):
+            raise KernelError(f"norms' weights, a gate's bias and a scale are contiguous float32 [{d}]")
     if (gate is None and gate_bias is not None) or (out is None and next_weight is not None):
         raise KernelError("a gate's bias needs a gate, and the next norm's weight rows to write")
     if T == 0 or d == 0 or (y is None and out is None and into is residual):
         return
     rc = _lib("norm_gate").qv_norm_gate_add(
-        _ptr(residual), _ptr(into), _ptr(y), _ld(y) if y is not None else d, dt_code(y.dtype) if y is not None else F32, _ptr(post_weight), float(post_eps),
-        _ptr(gate), _ld(gate) if gate is not None else d, dt_code(gate.dtype) if gate is not None else F32, _ptr(gate_bias), _ptr(scale), _ptr(next_weight),
-        float(next_eps), _ptr(o), (_ld16(o) if rows8 else _ld(o)) if o is not None else d, 2 if rows8 else dt_code(o.dtype) if o is not None else F32,
-        _ptr(out.scale) if rows8 else None, T, d, _stream())
+        residual.data_ptr(), into.data_ptr(), _ptr(y), ld_y, y_dt, _ptr(post_weight), post_eps, _ptr(gate), ld_gate, gate_dt, _ptr(gate_bias), _ptr(scale),
+        _ptr(next_weight), next_eps, _ptr(o), ld_out, out_kind, out.scale.data_ptr() if rows8 else None, T, d, _stream())
     _check(rc, "norm_gate_add")
+
+
+def _rows_of(t, shape, name: str):
+    """(row stride, type code) of a matrix of whole rows."""
+    strides = t.stride()
+    if t.shape != shape or (strides[1] != 1 and shape[1] > 1) or (shape[0] > 1 and strides[0] < shape[1]):
+        raise KernelError(f"{name} must be {tuple(shape)} with whole rows that do not overlap, not {tuple(t.shape)} with strides {strides}")
+    return (strides[0] if shape[0] > 1 else shape[1]), dt_code(t.dtype)
 
 
 # ------------------------------------------------------------------ attention
