@@ -52,12 +52,21 @@ struct Int8Args {
 // stay in L2; grouped: channels fastest, so that they share a tile's rows.
 #define BAND 16
 struct Item { int e, row0, rows, fb; };
-__device__ __forceinline__ Item item_at(const Int8Args& p, int item, int NT) {
+// What the table says of an item (nothing for a dense product), read an item ahead of its use: the trip to memory is then not waited for.
+struct Entry { int e, row0, rows; };
+__device__ __forceinline__ Entry entry_of(const Int8Args& p, int item, int items, int NT) {
+  Entry n = {-1, 0, 0};
+  if (p.tiles && item < items) {
+    const int* t = p.tiles + 3 * (item / NT);
+    n.e = t[0]; n.row0 = t[1]; n.rows = t[2];
+  }
+  return n;
+}
+__device__ __forceinline__ Item item_at(const Int8Args& p, const Entry& n, int item, int NT) {
   Item it;
   if (p.tiles) {
-    const int t = item / NT;
-    it.fb = item - t * NT;
-    it.e = p.tiles[3 * t]; it.row0 = p.tiles[3 * t + 1]; it.rows = p.tiles[3 * t + 2];
+    it.fb = item % NT;
+    it.e = n.e; it.row0 = n.row0; it.rows = n.rows;
     if (it.rows > p.bn) it.rows = p.bn;              // (a table that was made for other tiles or other rows reads and writes nothing outside)
     if (it.rows > p.rows - it.row0) it.rows = p.rows - it.row0;
     if (it.e >= p.experts || it.row0 < 0 || it.rows <= 0) it.e = -1;
@@ -71,7 +80,6 @@ __device__ __forceinline__ Item item_at(const Int8Args& p, int item, int NT) {
   it.rows = p.rows - it.row0 < p.bn ? p.rows - it.row0 : p.bn;
   return it;
 }
-
 
 // The gated activations (see GluAct) as g / (1 + exp(-a)) * u: the tanh form of GELU too, 1 + tanh(x) = 2 / (1 + exp(-2 x)), which loses
 // nothing where tanh is near -1.  Where the result is rounded to bfloat16 the fast exponential and quotient serve: their error, a few
@@ -156,13 +164,15 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
   pdl_wait();                                        // the rows, the tile table and the output belong to the kernels ahead until here
   const int NT = (p.N + BM - 1) / BM, NP = (NT + 1) / 2, KT = (p.K + QK - 1) / QK;
   const int items = p.row_tiles * NP, first = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  Entry entry = entry_of(p, first, items, NP);
 
   if (warp == 0) {
     const bool leader = elect_one();
     int it = 0;
     bool ok = true;
     for (int item = first; ok && item < items; item += pairs) {
-      const Item w = item_at(p, item, NP);
+      const Item w = item_at(p, entry, item, NP);
+      entry = entry_of(p, item + pairs, items, NP);
       if (w.e < 0) break;
       const int half = ((w.rows + 31) & ~31) >> 1;             // rows of either CTA
       const int boxes = (half + p.box - 1) / p.box;
@@ -190,7 +200,8 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
       int it = 0, local = 0;
       bool ok = true;
       for (int item = first; ok && item < items; item += pairs, ++local) {
-        const Item w = item_at(p, item, NP);
+        const Item w = item_at(p, entry, item, NP);
+      entry = entry_of(p, item + pairs, items, NP);
         if (w.e < 0) break;
         const uint32_t idesc = umma_idesc_i8(2 * BM, (w.rows + 31) & ~31);
         const int b = local & 1;
@@ -223,7 +234,8 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
     const uint32_t done[2] = {of_first(&acc_empty[0]), of_first(&acc_empty[1])};
     int local = 0;
     for (int item = first; item < items; item += pairs, ++local) {
-      const Item w = item_at(p, item, NP);
+      const Item w = item_at(p, entry, item, NP);
+      entry = entry_of(p, item + pairs, items, NP);
       if (w.e < 0) break;
       const int ch0 = (2 * w.fb + rank) * BM + q * 32;         // this warp's channels
       const float ws = ch0 + lane < p.N ? p.w_scale[(size_t)w.e * p.N + ch0 + lane] : 0.f;
@@ -245,24 +257,33 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
       for (int c0 = turn * 32; c0 < w.rows; c0 += 64) {
         uint32_t r[32];
         tmem_ld32(taddr + c0, r);
-        const float* sc = xs + (c0 >> 6) * 32;
+        float v[32];                                 // the rows' scales, then the scaled sums: all of them ahead of the first store
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) *(float4*)&v[j] = *(const float4*)(xs + (c0 >> 6) * 32 + j);
         tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * v[j] * ws;
         if (GLU) {
           // a lane of the lower half gives its gate value of the odd row for the up value of the even row
           const int up = lane >> 4;
           TO* o = out + (size_t)(c0 + up) * p.ld_out;
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const float a = (float)(int)r[j] * sc[j] * ws, c = (float)(int)r[j + 1] * sc[j + 1] * ws;
-            const float got = __shfl_xor_sync(0xffffffffu, up ? a : c, 16);
-            const float g = up ? got : a, u = up ? c : got;
-            if (c0 + j + up < w.rows && there) o[(size_t)j * p.ld_out] = from_f<TO>(gated<TO>(g, u, p.glu));
+            const float got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + 1], 16);
+            v[j] = gated<TO>(up ? got : v[j], up ? v[j + 1] : got, p.glu);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            if (c0 + j + up < w.rows && there) *o = from_f<TO>(v[j]);
+            o += 2 * p.ld_out;
           }
         } else if (there) {
           TO* o = out + (size_t)c0 * p.ld_out;
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c0 + j < w.rows) o[(size_t)j * p.ld_out] = from_f<TO>((float)(int)r[j] * sc[j] * ws);
+          for (int j = 0; j < 32; ++j) {
+            if (c0 + j < w.rows) *o = from_f<TO>(v[j]);
+            o += p.ld_out;
+          }
         }
         __syncwarp();
       }
@@ -297,7 +318,7 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
   uint64_t* empty = full + STAGES;
   uint64_t* accum = empty + STAGES;
   uint32_t* tmem_slot = (uint32_t*)(accum + 1);
-  __shared__ float xs[BN];                                     // the rows' scales
+  __shared__ __align__(16) float xs[BN];                       // the rows' scales
   int* sums = (int*)(ring + STAGES * STAGE_BYTES + 256);       // [splits][columns of this CTA / 4][128 channels][4]: what the cluster hands this CTA
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int KT = (p.K + QK - 1) / QK;
@@ -373,14 +394,26 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
   const bool there = warp >= 2 && (GLU ? 2 * feat < p.N : feat < p.N);
   TO* out = (TO*)p.out + (size_t)row0 * p.ld_out + feat;
   float ws = 0.f;
-  // a column's scaled sums to the output: all lanes of an epilogue warp are here
-  auto finish = [&](int c, int sum) {
-    const float v = (float)sum * xs[c] * ws;
+  // the scaled sums of columns c, c + 1, ... to the output: all lanes of an epilogue warp are here
+  auto finish = [&](int c, auto& sum) {
+    constexpr int N = sizeof(sum) / 4;
+    float v[N];                                      // all of them ahead of the first store
+#pragma unroll
+    for (int j = 0; j < N; j += 4) *(float4*)&v[j] = *(const float4*)&xs[c + j];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = (float)(int)sum[j] * v[j] * ws;
     if (GLU) {
-      const float other = __shfl_xor_sync(0xffffffffu, v, 16);
-      if (lane < 16 && there) out[(size_t)c * p.ld_out] = from_f<TO>(gated<TO>(v, other, p.glu));
-    } else if (there) {
-      out[(size_t)c * p.ld_out] = from_f<TO>(v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float other = __shfl_xor_sync(0xffffffffu, v[j], 16);
+        v[j] = gated<TO>(v[j], other, p.glu);        // (of the lower half; the upper half's are not stored)
+      }
+    }
+    TO* o = out + (size_t)c * p.ld_out;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (c + j < rows && there && (!GLU || lane < 16)) *o = from_f<TO>(v[j]);
+      o += p.ld_out;
     }
   };
   bool ok = true;
@@ -404,9 +437,7 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
       tmem_ld16(taddr + c0, r);
       tmem_wait_ld();
       if (p.splits == 1) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c0 + j < rows) finish(c0 + j, (int)r[j]);
+        finish(c0, r);
       } else {
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
@@ -429,16 +460,13 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
       for (int i = 0; i < mine; i += 4) {
         const int c = (split << shift) + i;
         if (c >= rows) break;
-        int4 t = make_int4(0, 0, 0, 0);
+        int t[4] = {0, 0, 0, 0};
 #pragma unroll 4
         for (int s = 0; s < p.splits; ++s) {
           const int4 v = part[((s << shift) + i) * (BM / 4)];
-          t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+          t[0] += v.x; t[1] += v.y; t[2] += v.z; t[3] += v.w;
         }
-        finish(c, t.x);
-        if (c + 1 < rows) finish(c + 1, t.y);
-        if (c + 2 < rows) finish(c + 2, t.z);
-        if (c + 3 < rows) finish(c + 3, t.w);
+        finish(c, t);
       }
     }
   }
@@ -603,35 +631,38 @@ int launch_pair_as(const CUtensorMap& map_x, const CUtensorMap& map_w, const Int
   return out_dt == QV_DT_BF16 ? launch_pair<false, bf16, RT, STAGES>(map_x, map_w, p, st) : launch_pair<false, float, RT, STAGES>(map_x, map_w, p, st);
 }
 
-// CTAs that share a block of channels (1, 2 or 4), of at least 4 k blocks each: as many as the SMs hold at once, and up to 64 rows, whose sums
-// are cheap to hand over, a third more.  us with 1 / 2 / 4 / 8: 4096 x 14336, 1 row 22.1 / 14.0 / 12.9 / 12.6, 64 rows 30.6 / 23.7 / 17.5 / 21.1;
-// 2048 x 8192, 8 rows 14.0 / 9.8 / 7.4 / 10.7; 6144 x 4096 (48 blocks), 8 rows 9.2 / 8.4 / 8.1 / 9.7, 64 rows 12.7 / 12.1 / 11.0 / 15.5, 77 rows
-// 15.9 / 16.2 / 19.3; 28672 x 4096, 8 rows 22.4 / 25.5 / 26.5.
-int few_splits(int blocks, int rows, int KT, int sms) {
-  int splits = 1;
-  const int most = rows <= 64 ? sms + sms / 3 : sms;
-  while (splits < 4 && blocks * splits * 2 <= most && KT >= splits * 8) splits *= 2;
-#ifdef INT8_PROBE
-  if (getenv("QF_S")) return atoi(getenv("QF_S"));
-#endif
-  return splits;
-}
-
-// Whether the kernel for few rows takes a dense product: up to 64 rows, and up to 128 where four CTAs a block of channels find room (128 rows, 4096 x
-// 14336: 24.0 us against the pairs' 32.0; 77 rows, 6144 x 4096, where they do not: 16.1 against 12.8).
-bool few_rows(int rows, int N, int sms) { return rows <= 64 || (rows <= 128 && (N + BM - 1) / BM * 4 <= sms); }
-
-// Rows of the pairs' tiles, a multiple of 32: of the widths that need the least time, rounds of items times that of an item, the largest.  A k
-// block takes a pair 187 ns up to 64 rows, 235 at 128, 303 at 192 and 387 at 256 (2,048 rows, 28672 x 4096): what the SMs take in.
-int tile_rows_of(int rows, int N, int pairs) {
-  long long best = 0;
-  int width = 32;
-  for (int bn = 32; bn <= 256; bn += 32) {
-    const long long items = (long long)((rows + bn - 1) / bn) * ((N + 2 * BM - 1) / (2 * BM));
-    const long long cost = (items + pairs - 1) / pairs * ((bn < 64 ? 64 : bn) + 116);
-    if (bn == 32 || cost <= best) { best = cost; width = bn; }
+// How a dense product is cut, by the time that each cut is expected to take: rounds of CTAs or pairs, times the k blocks of one, times what an
+// SM takes in for a k block at 88 bytes a ns, plus what comes behind.
+//   few rows: tiles of 16, 32 or 64 rows, 1, 2 or 4 CTAs that share a block of channels, two CTAs an SM; a tile's last stores and, with several
+//     CTAs, handing over its sums cost some 20 and 15 ns a row.
+//   pairs: tiles of a multiple of 32 rows; a k block takes 187 ns up to 64 rows, 235 at 128, 303 at 192 and 387 at 256 (2,048 rows, 28672 x
+//     4096); 3.5 us for setting up pairs, and for filling and emptying them.
+// Measured, us with their rounding to 8 bits (few as rows / CTAs): 77 rows, 777 x 1001: 16/1 4.9, 16/2 4.7, 32/4 4.6, 64/1 5.9, pairs of 32 6.1; 128
+// rows, 4096 x 14336: 32/2 21.9, 64/2 18.8, 64/4 18.9, pairs of 64 26.3; 256 rows, 2048 x 2048: 16/1 7.2, 32/1 7.1, 64/2 8.0, pairs of 64 7.9;
+// 512 rows, 1024 x 1024: 32/1 5.4, pairs of 64 6.5; 64 rows, 28672 x 4096: 64/1 28.5, pairs of 64 26.3; 8 rows of it: 16/1 22.1, pairs of 32 24.5.
+struct Plan { int few, bn, splits; };
+Plan plan_of(int rows, int N, int K, int sms) {
+  const long long KT = (K + QK - 1) / QK, blocks = (N + BM - 1) / BM, pairs = sms / 2;
+  Plan best = {1, 16, 1};
+  long long least = 0x7fffffffffffffffLL;
+  for (int bn = 16; bn <= 64; bn *= 2) {
+    if (bn > 16 && bn / 2 >= rows) break;
+    const long long tiles = (rows + bn - 1) / bn;
+    if (tiles > 65535) continue;
+    for (int splits = 1; splits <= 4; splits *= 2) {
+      const long long ctas = blocks * tiles * splits;
+      if (splits > 1 && (ctas > 2 * sms || KT < 2 * splits)) break;
+      const long long cost = (ctas + sms - 1) / sms * ((KT + splits - 1) / splits) * (128 + bn) * 145 / 100 + 20 * bn + (splits > 1 ? 800 + 15 * bn : 0);
+      if (cost <= least) { least = cost; best = {1, bn, splits}; }
+    }
   }
-  return width;
+  for (int bn = 32; bn <= 256; bn += 32) {
+    if (bn > 32 && bn - 32 >= rows) break;
+    const long long items = (rows + bn - 1) / bn * ((N + 2 * BM - 1) / (2 * BM));
+    const long long cost = (items + pairs - 1) / pairs * KT * ((bn < 64 ? 64 : bn) + 116) * 104 / 100 + 3500;
+    if (cost < least || (!best.few && cost == least)) { least = cost; best = {0, bn, 1}; }
+  }
+  return best;
 }
 
 template <bool GLU, typename TO, int BN, int STAGES>
@@ -652,11 +683,11 @@ int launch_few(const CUtensorMap& map, Int8Args p, int blocks, int tiles, cudaSt
 template <int BN, int DEEP, int SHALLOW>
 int launch_few_as(const CUtensorMap& map, Int8Args p, bool glu, int out_dt, cudaStream_t st) {
   const int blocks = (p.N + BM - 1) / BM, KT = (p.K + QK - 1) / QK, tiles = (p.rows + BN - 1) / BN, sms = sms_of_device();
-  if (tiles > 65535) return QV_ERR_TOO_LARGE;
-  const int splits = few_splits(blocks * tiles, p.rows, KT, sms);
-  p.kb_per_split = (KT + splits - 1) / splits;
-  p.splits = (KT + p.kb_per_split - 1) / p.kb_per_split;       // none without k blocks
-  const bool one_wave = (long long)blocks * tiles * p.splits <= sms;
+  p.kb_per_split = (KT + p.splits - 1) / p.splits;
+  while ((p.splits - 1) * p.kb_per_split >= KT) p.splits /= 2, p.kb_per_split = (KT + p.splits - 1) / p.splits;      // none without k blocks
+  // a ring that fills the SM where every CTA finds one for itself (clusters of four find 32 places on 148 SMs), else two CTAs an SM
+  const long long ctas = (long long)blocks * tiles * p.splits;
+  const bool one_wave = p.splits == 4 ? ctas * 8 <= sms * 7 : ctas <= sms;
 #define FEW(GLU, TO) return one_wave ? launch_few<GLU, TO, BN, DEEP>(map, p, blocks, tiles, st) : launch_few<GLU, TO, BN, SHALLOW>(map, p, blocks, tiles, st)
   if (glu) {
     if (out_dt == QV_DT_BF16) FEW(true, bf16);
@@ -728,27 +759,19 @@ extern "C" int qv_gemm_int8(void* out, long long ld_out, int out_dt, const int8_
   p.glu = {glu ? act : 0, limit, slope};
   cudaStream_t st = (cudaStream_t)stream;
   CUtensorMap map, map_w;
-  int few = few_rows(rows, N, sms_of_device());
-#ifdef INT8_PROBE
-  if (getenv("QF_T")) few = rows <= atoi(getenv("QF_T"));
-#endif
-  if (!tiles && few) {
-    const int bn = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-    if (!make_map_i8(&map, x, rows, K, ld_x, bn)) return QV_ERR_UNSUPPORTED;
-    if (bn == 16) return launch_few_as<16, 10, 5>(map, p, glu, out_dt, st);
-    if (bn == 32) return launch_few_as<32, 9, 4>(map, p, glu, out_dt, st);
-    if (bn == 64) return launch_few_as<64, 7, 3>(map, p, glu, out_dt, st);
-    return launch_few_as<128, 4, 3>(map, p, glu, out_dt, st);
-  }
   int rt;
   if (tiles) {
     if (max_tiles <= 0) return 0;
     rt = tile_rows; p.bn = tile_rows; p.row_tiles = max_tiles; p.box = 16;
   } else {
-    p.bn = tile_rows_of(rows, N, sms_of_device() / 2);
-#ifdef INT8_PROBE
-    if (getenv("QF_BN")) p.bn = atoi(getenv("QF_BN"));
-#endif
+    const Plan plan = plan_of(rows, N, K, sms_of_device());
+    p.bn = plan.bn; p.splits = plan.splits;
+    if (plan.few) {
+      if (!make_map_i8(&map, x, rows, K, ld_x, p.bn)) return QV_ERR_UNSUPPORTED;
+      if (p.bn == 16) return launch_few_as<16, 10, 5>(map, p, glu, out_dt, st);
+      if (p.bn == 32) return launch_few_as<32, 9, 4>(map, p, glu, out_dt, st);
+      return launch_few_as<64, 7, 3>(map, p, glu, out_dt, st);
+    }
     rt = p.bn <= 32 ? 32 : p.bn <= 64 ? 64 : p.bn <= 128 ? 128 : 256;
     p.box = p.bn / 2; p.row_tiles = (rows + p.bn - 1) / p.bn;
   }
