@@ -62,7 +62,7 @@ EXTRA_SOURCES = {
     "host_runtime": ["host/dispatch.hpp"],
     "gemm_simt": ["per_device.h"],
     "gemm_int8": ["int8_rows.cuh", "per_device.h"],
-    "norm_gate": ["int8_rows.cuh"],
+    "norm_gate": ["int8_rows.cuh", "per_device.h"],
     "recurrent": ["portion_rounds.h", "per_device.h"],
     "channel_scan": ["portion_rounds.h", "per_device.h"],
     "executor": ["host/executor.hpp", "host/kernels.hpp", "host/dispatch.hpp"],

@@ -551,8 +551,9 @@ __global__ void __launch_bounds__(WARP ? 32 * QUANTIZE_WARPS : 1024) quantize_ro
     for (int i = 0; i < VECS; ++i) top = larger(top, v[i], xr);
   }
   top = top_bits(top, xr);
-  const Int8Scale s = int8_scale(WARP ? __uint_as_float(__reduce_max_sync(0xffffffffu, top)) : int8_block_top(top, red));
-  if (at == 0) scale[r] = s.scale;
+  const float most = WARP ? __uint_as_float(__reduce_max_sync(0xffffffffu, top)) : int8_block_top(top, red);
+  const Int8Scale s = int8_scale(most);
+  if (at == 0) scale[r] = int8_step(most);
   if (LONG) {
     for (int k = at; k < K; k += step) store_piece<T>(o, load_piece<T, ALIGNED>(xr, k, n), s, k, K);
   } else {
@@ -577,16 +578,6 @@ __global__ void __launch_bounds__(256) pack_int8_kernel(uint4* __restrict__ out,
 }
 
 // ---------------------------------------------------------------- host side
-int sms_of_device() {
-  static std::atomic<int> known[64];
-  int dev = 0, v = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (dev >= 0 && dev < 64 && (v = known[dev].load(std::memory_order_relaxed)) > 0) return v;
-  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) v = 148;
-  if (dev >= 0 && dev < 64) known[dev].store(v, std::memory_order_relaxed);
-  return v;
-}
-
 // Rows of 8-bit integers [rows, K], row stride ld bytes; box = 128 k x box_rows, 128-byte swizzle, zeros outside.
 bool make_map_i8(CUtensorMap* map, const void* ptr, long long rows, int K, long long ld, int box_rows) {
   EncodeTiledFn fn = encode_fn();
@@ -621,7 +612,7 @@ int launch_pair(const CUtensorMap& map_x, const CUtensorMap& map_w, const Int8Ar
   if (rc) return rc;
   const long long items = (long long)p.row_tiles * ((p.N + 2 * BM - 1) / (2 * BM));
   if (items > 0x40000000LL) return QV_ERR_TOO_LARGE;
-  const int pairs = sms_of_device() / 2;
+  const int pairs = device_sms() / 2;
   return qv_launch_cluster(kernel, dim3(2 * (unsigned)(items < pairs ? items : pairs)), dim3(PAIR_THREADS), (size_t)smem, st, dim3(2, 1, 1), map_x, map_w, p);
 }
 
@@ -682,7 +673,7 @@ int launch_few(const CUtensorMap& map, Int8Args p, int blocks, int tiles, cudaSt
 
 template <int BN, int DEEP, int SHALLOW>
 int launch_few_as(const CUtensorMap& map, Int8Args p, bool glu, int out_dt, cudaStream_t st) {
-  const int blocks = (p.N + BM - 1) / BM, KT = (p.K + QK - 1) / QK, tiles = (p.rows + BN - 1) / BN, sms = sms_of_device();
+  const int blocks = (p.N + BM - 1) / BM, KT = (p.K + QK - 1) / QK, tiles = (p.rows + BN - 1) / BN, sms = device_sms();
   p.kb_per_split = (KT + p.splits - 1) / p.splits;
   while ((p.splits - 1) * p.kb_per_split >= KT) p.splits /= 2, p.kb_per_split = (KT + p.splits - 1) / p.splits;      // none without k blocks
   // a ring that fills the SM where every CTA finds one for itself (clusters of four find 32 places on 148 SMs), else two CTAs an SM
@@ -734,7 +725,7 @@ extern "C" int qv_quantize_rows(int8_t* q, long long ld_q, float* scale, const v
   } while (0)
   QV_DISPATCH_DT(x_dt, TX, {
     const int pieces = (K + Piece<TX>::N - 1) / Piece<TX>::N;
-    const bool few = T <= 2 * sms_of_device();                  // blocks of as many threads as a row has pieces find room at once
+    const bool few = T <= 2 * device_sms();                  // blocks of as many threads as a row has pieces find room at once
     if (((uintptr_t)x & 15) == 0 && (ld_x * sizeof(TX)) % 16 == 0) QUANTIZE_AS(true);
     QUANTIZE_AS(false);
   });
@@ -764,7 +755,7 @@ extern "C" int qv_gemm_int8(void* out, long long ld_out, int out_dt, const int8_
     if (max_tiles <= 0) return 0;
     rt = tile_rows; p.bn = tile_rows; p.row_tiles = max_tiles; p.box = 16;
   } else {
-    const Plan plan = plan_of(rows, N, K, sms_of_device());
+    const Plan plan = plan_of(rows, N, K, device_sms());
     p.bn = plan.bn; p.splits = plan.splits;
     if (plan.few) {
       if (!make_map_i8(&map, x, rows, K, ld_x, p.bn)) return QV_ERR_UNSUPPORTED;

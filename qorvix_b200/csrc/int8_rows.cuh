@@ -10,22 +10,24 @@
 // What is rounded has then lost half a step of 1/127 of the row's largest entry, no more.
 #pragma once
 #include "common.cuh"
+#include <atomic>
 
 struct Int8Scale {
   float top, pre, inv;        // the largest magnitude and the entries times `pre`, a power of two that keeps 127 / top in range
-  float scale;
   bool live;                  // false: all q are 0
 };
 
 __device__ __forceinline__ Int8Scale int8_scale(float top) {
   Int8Scale s;
   s.live = top > 0.f && top < __int_as_float(0x7f800000);
-  s.scale = __fdiv_rn(top, 127.f);
-  if (!(top < __int_as_float(0x7f800000))) s.scale = __int_as_float(0x7fffffff);
   s.pre = top < 0x1p-60f ? 0x1p64f : top > 0x1p60f ? 0x1p-64f : 1.f;
   s.top = top * s.pre;        // exact: entries that fall below the normal range are under 2^-60 of top
   s.inv = s.live ? __fdiv_rn(127.f, s.top) : 0.f;
   return s;
+}
+// What is kept beside the row: top / 127, of which the row's entries are whole multiples.
+__device__ __forceinline__ float int8_step(float top) {
+  return top < __int_as_float(0x7f800000) ? __fdiv_rn(top, 127.f) : __int_as_float(0x7fffffff);
 }
 
 // The row's entry x (times s.pre), whose quotient lies next to the border on the side d of the number r that t = r + 1.5 2^23 holds: whether it
@@ -114,4 +116,15 @@ __device__ __forceinline__ float int8_block_top(uint32_t bits, uint32_t* red /* 
   if (lane == 0) red[warp] = bits;
   __syncthreads();
   return __uint_as_float(__reduce_max_sync(0xffffffffu, lane < nwarp ? red[lane] : 0u));
+}
+
+// Streaming multiprocessors of the current device.
+static inline int device_sms() {
+  static std::atomic<int> known[64];
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < 64 && (v = known[dev].load(std::memory_order_relaxed)) > 0) return v;
+  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) v = 148;
+  if (dev >= 0 && dev < 64) known[dev].store(v, std::memory_order_relaxed);
+  return v;
 }

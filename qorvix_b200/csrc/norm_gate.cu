@@ -10,6 +10,8 @@
 // rms(v) = sqrt(mean(v^2) + eps).  Sums and everything between are float32.  8-bit rows are those of the bfloat16 rows, so that they do
 // not depend on whether this pass or qv_quantize_rows made them.
 #include "int8_rows.cuh"
+#include "per_device.h"
+#include "tc_common.cuh"
 #include <type_traits>
 
 namespace {
@@ -59,7 +61,7 @@ template <typename T, bool ALIGNED> __device__ __forceinline__ void store_four(T
   if (i + 2 < d) p[i + 2] = from_f<T>(v.z);
   if (i + 3 < d) p[i + 3] = from_f<T>(v.w);
 }
-__device__ __forceinline__ float sigmoid_of(float v) { return 1.0f / (1.0f + __expf(-v)); }
+__device__ __forceinline__ float sigmoid_of(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }      // within a few steps of 2^-23
 __device__ __forceinline__ float square_sum(float4 v) { return (v.x * v.x + v.y * v.y) + (v.z * v.z + v.w * v.w); }
 __device__ __forceinline__ float4 mul(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
 __device__ __forceinline__ float4 mul(float4 a, float b) { return make_float4(a.x * b, a.y * b, a.z * b, a.w * b); }
@@ -75,6 +77,41 @@ __device__ __forceinline__ float block_total(float v, float* red /* >= 32 */) {
   return warp_sum(lane < nwarp ? red[lane] : 0.f);
 }
 
+// What the row-wide operands hold beside one group of four: post is the norm's weight times the scale; ones (a bias: zeros) stand for what there
+// is not, which changes no bit.
+struct Beside { float4 post, bias; };
+struct NoGate {};                                            // in the place of the gate's type
+__device__ __forceinline__ float4 four_of(float v) { return make_float4(v, v, v, v); }
+template <typename TG, bool ALIGNED> __device__ __forceinline__ Beside beside(const NormGateArgs& a, int i) {
+  Beside w;
+  w.post = a.w_post ? load_four<float, ALIGNED>(a.w_post, i, a.d) : four_of(1.f);
+  if (a.scale) w.post = mul(w.post, load_four<float, ALIGNED>(a.scale, i, a.d));
+  if constexpr (!std::is_same<TG, NoGate>::value) w.bias = a.gate_bias ? load_four<float, ALIGNED>(a.gate_bias, i, a.d) : four_of(0.f);
+  return w;
+}
+template <typename TG, bool ALIGNED> __device__ __forceinline__ float4 load_gate(const TG* g, int i, int d) {
+  if constexpr (std::is_same<TG, NoGate>::value) return make_float4(0.f, 0.f, 0.f, 0.f);
+  else return load_four<TG, ALIGNED>(g, i, d);
+}
+// The new stream's entries: x + z (times 1 / rms(y), and the norm's weight times the scale) (times the gate).
+template <typename TG> __device__ __forceinline__ float4 new_stream(float4 x, float4 z, float4 g, float inv_rms, const Beside& w) {
+  z = mul(mul(z, inv_rms), w.post);
+  if constexpr (!std::is_same<TG, NoGate>::value)
+    z = mul(z, make_float4(sigmoid_of(g.x + w.bias.x), sigmoid_of(g.y + w.bias.y), sigmoid_of(g.z + w.bias.z), sigmoid_of(g.w + w.bias.w)));
+  return make_float4(x.x + z.x, x.y + z.y, x.z + z.z, x.w + z.w);
+}
+__device__ __forceinline__ float4 rounded(float4 v) {
+  return make_float4(to_f(from_f<bf16>(v.x)), to_f(from_f<bf16>(v.y)), to_f(from_f<bf16>(v.z)), to_f(from_f<bf16>(v.w)));
+}
+__device__ __forceinline__ uint32_t larger(uint32_t top, float4 v) { return max(top, max(max(int8_bits(v.x), int8_bits(v.y)), max(int8_bits(v.z), int8_bits(v.w)))); }
+__device__ __forceinline__ void put_int8(int8_t* o, int i, int d, float4 v, const Int8Scale& s) {
+  float f[4] = {v.x, v.y, v.z, v.w};
+  uint32_t w[1];
+  int8_pack<true, 4>(f, s, w);
+  if (i + 4 <= d) { *(uint32_t*)(o + i) = w[0]; return; }
+  for (int k = 0; i + k < d; ++k) o[i + k] = (int8_t)(w[0] >> (8 * k));
+}
+
 // A block a row, FOURS groups of four entries a thread, in registers from the first load to the last store: each operand is read once and all
 // loads of a row are in flight together (two sums over the row lie between them and the stores).  LONG: rows longer than four groups of
 // 512 threads, of which the new stream is read back from where this thread stored it.
@@ -88,24 +125,11 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
   const float* sr = a.stream + (size_t)t * d;
   float* so = a.into + (size_t)t * d;
   const TY* yr = a.y ? (const TY*)a.y + (size_t)t * a.ld_y : nullptr;
-  const TG* gr = a.gate ? (const TG*)a.gate + (size_t)t * a.ld_gate : nullptr;
+  const TG* gr = (const TG*)a.gate + (std::is_same<TG, NoGate>::value ? 0 : (size_t)t * a.ld_gate);
   float4 x[FOURS], z[FOURS], g[FOURS];
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 next_of_one = zero;
   float post = 1.f, s2 = 0.f;
-  // the new stream's entries from what was read
-  auto add = [&](int i, float4 x, float4 z, float4 g) {
-    if (!yr) return x;
-    if (a.w_post) z = mul(mul(z, post), load_four<float, ALIGNED>(a.w_post, i, d));
-    if (gr) {
-      if (a.gate_bias) {
-        const float4 b = load_four<float, ALIGNED>(a.gate_bias, i, d);
-        g = make_float4(g.x + b.x, g.y + b.y, g.z + b.z, g.w + b.w);
-      }
-      z = mul(z, make_float4(sigmoid_of(g.x), sigmoid_of(g.y), sigmoid_of(g.z), sigmoid_of(g.w)));
-    }
-    if (a.scale) z = mul(z, load_four<float, ALIGNED>(a.scale, i, d));
-    return make_float4(x.x + z.x, x.y + z.y, x.z + z.z, x.w + z.w);
-  };
   const bool stores = yr != nullptr || so != sr;
   if (LONG) {
     if (yr && a.w_post) {
@@ -114,7 +138,8 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
       post = 1.0f / sqrtf(block_total(ss, red) / (float)d + a.eps_post);
     }
     for (int i = threadIdx.x * 4; i < d; i += step) {
-      const float4 v = add(i, load_four<float, ALIGNED>(sr, i, d), yr ? load_four<TY, ALIGNED>(yr, i, d) : zero, gr ? load_four<TG, ALIGNED>(gr, i, d) : zero);
+      const float4 v = new_stream<TG>(load_four<float, ALIGNED>(sr, i, d), yr ? load_four<TY, ALIGNED>(yr, i, d) : zero, load_gate<TG, ALIGNED>(gr, i, d), post,
+                                      beside<TG, ALIGNED>(a, i));
       if (stores) store_four<float, ALIGNED>(so, i, d, v);
       s2 += square_sum(v);
     }
@@ -125,8 +150,15 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
       const bool in = i < d;
       z[k] = in && yr ? load_four<TY, ALIGNED>(yr, i, d) : zero;
       x[k] = in ? load_four<float, ALIGNED>(sr, i, d) : zero;
-      g[k] = in && gr ? load_four<TG, ALIGNED>(gr, i, d) : zero;
+      g[k] = in ? load_gate<TG, ALIGNED>(gr, i, d) : zero;
     }
+    Beside w[FOURS];                                 // of one group: on its way with the row, ahead of the sum
+    float4 w_next = zero;
+    if (FOURS == 1 && threadIdx.x * 4 < d) {
+      w[0] = beside<TG, ALIGNED>(a, threadIdx.x * 4);
+      if (a.w_next) w_next = load_four<float, ALIGNED>(a.w_next, threadIdx.x * 4, d);
+    }
+    next_of_one = w_next;
     if (yr && a.w_post) {
       float ss = 0.f;
 #pragma unroll
@@ -137,7 +169,7 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
     for (int k = 0; k < FOURS; ++k) {
       const int i = threadIdx.x * 4 + k * step;
       if (i < d) {
-        x[k] = add(i, x[k], z[k], g[k]);
+        x[k] = new_stream<TG>(x[k], z[k], g[k], post, FOURS == 1 ? w[0] : beside<TG, ALIGNED>(a, i));
         if (stores) store_four<float, ALIGNED>(so, i, d, x[k]);
         s2 += square_sum(x[k]);
       }
@@ -145,9 +177,8 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
   }
   if (!a.out) return;
   const float next = a.w_next ? 1.0f / sqrtf(block_total(s2, red) / (float)d + a.eps_next) : 1.f;
-  auto row = [&](int i, float4 v) { return a.w_next ? mul(mul(v, next), load_four<float, ALIGNED>(a.w_next, i, d)) : v; };
-  auto rounded = [&](float4 v) {
-    return make_float4(to_f(from_f<bf16>(v.x)), to_f(from_f<bf16>(v.y)), to_f(from_f<bf16>(v.z)), to_f(from_f<bf16>(v.w)));
+  auto row = [&](int i, float4 v) {
+    return a.w_next ? mul(mul(v, next), FOURS == 1 && !LONG ? next_of_one : load_four<float, ALIGNED>(a.w_next, i, d)) : v;
   };
   const float* nr = stores ? so : sr;
   if (OUT != 2) {
@@ -165,47 +196,170 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
     return;
   }
   uint32_t top = 0;
-  auto larger = [&](float4 v) { top = max(top, max(max(int8_bits(v.x), int8_bits(v.y)), max(int8_bits(v.z), int8_bits(v.w)))); };
   if (LONG) {
-    for (int i = threadIdx.x * 4; i < d; i += step) larger(rounded(row(i, load_four<float, ALIGNED>(nr, i, d))));
+    for (int i = threadIdx.x * 4; i < d; i += step) top = larger(top, rounded(row(i, load_four<float, ALIGNED>(nr, i, d))));
   } else {
 #pragma unroll
     for (int k = 0; k < FOURS; ++k) {
       const int i = threadIdx.x * 4 + k * step;
       if (i < d) {
         x[k] = rounded(row(i, x[k]));
-        larger(x[k]);
+        top = larger(top, x[k]);
       }
     }
   }
-  const Int8Scale s = int8_scale(int8_block_top(top, (uint32_t*)red));
-  if (threadIdx.x == 0) a.out_scale[t] = s.scale;
+  const float most = int8_block_top(top, (uint32_t*)red);
+  const Int8Scale s = int8_scale(most);
+  if (threadIdx.x == 0) a.out_scale[t] = int8_step(most);
   int8_t* o = (int8_t*)a.out + (size_t)t * a.ld_out;
-  auto put = [&](int i, float4 v) {
-    float f[4] = {v.x, v.y, v.z, v.w};
-    uint32_t w[1];
-    int8_pack<true, 4>(f, s, w);
-    if (i + 4 <= d) { *(uint32_t*)(o + i) = w[0]; return; }
-    for (int k = 0; i + k < d; ++k) o[i + k] = (int8_t)(w[0] >> (8 * k));
-  };
   if (LONG) {
-    for (int i = threadIdx.x * 4; i < d; i += step) put(i, rounded(row(i, load_four<float, ALIGNED>(nr, i, d))));
+    for (int i = threadIdx.x * 4; i < d; i += step) put_int8(o, i, d, rounded(row(i, load_four<float, ALIGNED>(nr, i, d))), s);
   } else {
 #pragma unroll
     for (int k = 0; k < FOURS; ++k) {
       const int i = threadIdx.x * 4 + k * step;
-      if (i < d) put(i, x[k]);
+      if (i < d) put_int8(o, i, d, x[k], s);
     }
   }
 }
 
+// Many rows: what bounds the pass is memory, so an SM should never be without loads on the way.  As many blocks as the SMs hold walk over the
+// rows; the rows ahead of the one that a block works on come into shared memory by bulk copies, a ring of `stages` of them (two or more), and the weights,
+// which all rows share, stay in registers.  A row then costs two sums over the block (a barrier each) and its arithmetic.  Every row of
+// every operand on 16 bytes and a multiple of them, rows of up to FOURS groups of THREADS threads, as many blocks on an SM as make 1,280 threads:
+// one block's sums and stores run beside another's.
+// 2,048 rows of 5,120, bfloat16 y, gate and rows: 26.7 us, 5.5 TB/s; 53 with a block a row, which waits for its loads and its sums in turn, 46 with
+// the next row on its way to registers, 33 with weights that took more registers than two blocks find.  The stages do not matter from two on.
+__device__ __forceinline__ float block_total_of(float v, float* red /* >= 32; read by all since this row's or the last row's barrier */) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
+  v = warp_sum(v);
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  return warp_sum(lane < nwarp ? red[lane] : 0.f);
+}
+template <typename TY, typename TG, int OUT, int FOURS, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS) norm_gate_rows_kernel(const NormGateArgs a, int T, int stages, float inv_d, int* err) {
+  extern __shared__ __align__(128) uint8_t ring[];           // [stages][stream row | y row | gate row]
+  __shared__ float red[4][32];                               // of the first sum, the second in rows of either parity, the maximum
+  __shared__ uint64_t full[8];
+  const int d = a.d, n4 = d / 4, step = blockDim.x;
+  const bool has_y = a.y != nullptr, has_post = has_y && a.w_post, has_next = a.w_next != nullptr;
+  const uint32_t x_bytes = d * 4, y_bytes = has_y ? d * (uint32_t)sizeof(TY) : 0, g_bytes = std::is_same<TG, NoGate>::value ? 0 : d * (uint32_t)sizeof(TG);
+  const uint32_t stage_bytes = x_bytes + y_bytes + g_bytes;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+  pdl_wait();
+  auto fetch = [&](int t, int s) {                           // by thread 0
+    uint8_t* dst = ring + s * stage_bytes;
+    mbar_expect_tx(&full[s], stage_bytes);
+    bulk_load_1d(dst, a.stream + (size_t)t * d, &full[s], x_bytes);
+    if (y_bytes) bulk_load_1d(dst + x_bytes, (const TY*)a.y + (size_t)t * a.ld_y, &full[s], y_bytes);
+    if (g_bytes) bulk_load_1d(dst + x_bytes + y_bytes, (const TG*)a.gate + (size_t)t * a.ld_gate, &full[s], g_bytes);
+  };
+  if (threadIdx.x == 0)
+    for (int s = 0; s < stages; ++s)
+      if (blockIdx.x + s * gridDim.x < T) fetch(blockIdx.x + s * gridDim.x, s);
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  Beside w[FOURS];
+  float4 wn[FOURS];
+#pragma unroll
+  for (int k = 0; k < FOURS; ++k) {
+    const int i = threadIdx.x + k * step;
+    w[k] = i < n4 ? beside<TG, true>(a, 4 * i) : Beside{zero, zero};
+    wn[k] = i < n4 && has_next ? ((const float4*)a.w_next)[i] : four_of(1.f);
+  }
+  const bool stores = has_y || a.into != a.stream;
+  bool ok = true;                                            // false: a wait gave up; the rest of this block's rows say nothing, and the error word does
+  int it = 0;
+  for (int t = blockIdx.x; t < T; t += gridDim.x, ++it) {
+    const int s = it % stages;
+    const uint8_t* row = ring + s * stage_bytes;
+    ok = ok && mbar_wait(&full[s], (it / stages) & 1, err, 71);
+    float post = 1.f, s2 = 0.f;
+    if (has_post) {
+      float ss = 0.f;
+#pragma unroll
+      for (int k = 0; k < FOURS; ++k)
+        if (threadIdx.x + k * step < n4) ss += square_sum(Four<TY>::load((const TY*)(row + x_bytes) + 4 * (threadIdx.x + k * step)));
+      post = rsqrtf(block_total_of(ss, red[0]) * inv_d + a.eps_post);
+    }
+    float4 v[FOURS];
+#pragma unroll
+    for (int k = 0; k < FOURS; ++k) {
+      const int i = threadIdx.x + k * step;
+      v[k] = zero;
+      if (i < n4) {
+        v[k] = ((const float4*)row)[i];
+        if (has_y) v[k] = new_stream<TG>(v[k], Four<TY>::load((const TY*)(row + x_bytes) + 4 * i), load_gate<TG, true>((const TG*)(row + x_bytes + y_bytes), 4 * i, d), post, w[k]);
+        s2 += square_sum(v[k]);
+        if (stores) ((float4*)(a.into + (size_t)t * d))[i] = v[k];
+      }
+    }
+    const float total = block_total_of(s2, red[1 + (it & 1)]), next = has_next ? rsqrtf(total * inv_d + a.eps_next) : 1.f;
+    if (threadIdx.x == 0 && t + (long long)stages * gridDim.x < T) fetch(t + stages * gridDim.x, s);      // (behind the barrier: the row has been read)
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < FOURS; ++k) {
+      const int i = threadIdx.x + k * step;
+      if (a.out && i < n4) {
+        v[k] = mul(mul(v[k], next), wn[k]);
+        if (OUT == 0) Four<float>::store((float*)a.out + (size_t)t * a.ld_out + 4 * i, v[k]);
+        if (OUT == 1) Four<bf16>::store((bf16*)a.out + (size_t)t * a.ld_out + 4 * i, v[k]);
+        if (OUT == 2) {
+          v[k] = rounded(v[k]);
+          top = larger(top, v[k]);
+        }
+      }
+    }
+    if (OUT == 2) {
+      const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) red[3][warp] = __uint_as_float(top);
+      __syncthreads();
+      const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < nwarp ? __float_as_uint(red[3][lane]) : 0u));
+      const Int8Scale q = int8_scale(most);
+      if (threadIdx.x == 0) a.out_scale[t] = int8_step(most);
+#pragma unroll
+      for (int k = 0; k < FOURS; ++k)
+        if (threadIdx.x + k * step < n4) put_int8((int8_t*)a.out + (size_t)t * a.ld_out, 4 * (threadIdx.x + k * step), d, v[k], q);
+    }
+  }
+}
+
+template <typename TY, typename TG, int OUT, int FOURS, int THREADS>
+int launch_norm_gate_rows(const NormGateArgs& a, int T, int sms, int* err, cudaStream_t st) {
+  static PerDevice devices;
+  constexpr int ROOM = 216 * 1024;
+  auto kernel = norm_gate_rows_kernel<TY, TG, OUT, FOURS, THREADS>;
+  const int rc = qv_allow_smem(kernel, ROOM, devices);
+  if (rc) return rc;
+  const int threads = (a.d / 4 + 32 * FOURS - 1) / (32 * FOURS) * 32;
+  const int on_sm = 1280 / THREADS, blocks = sms * on_sm;
+  const size_t stage = (size_t)a.d * (4 + (a.y ? sizeof(TY) : 0) + (std::is_same<TG, NoGate>::value ? 0 : sizeof(TG)));
+  int stages = (int)((size_t)ROOM / on_sm / stage);
+  stages = stages > 6 ? 6 : stages;
+  return qv_launch(kernel, dim3(T < blocks ? T : blocks), dim3(threads), stages * stage, st, a, T, stages, 1.0f / (float)a.d, err);
+}
+
 template <typename TY, typename TG, int OUT, bool ALIGNED>
-int launch_norm_gate(const NormGateArgs& a, int T, cudaStream_t st) {
-  const int fours = (a.d + 3) / 4;
+int launch_norm_gate(const NormGateArgs& a, int T, int* err, cudaStream_t st) {
+  const int fours = (a.d + 3) / 4, sms = device_sms();
+  // whole 16-byte pieces in every row that a bulk copy brings
+  const bool pieces = ((uintptr_t)a.y & 15) == 0 && ((uintptr_t)a.gate & 15) == 0 && (a.d * sizeof(TY)) % 16 == 0 && (!a.gate || ((a.d * sizeof(TG)) % 16 == 0 && (a.ld_gate * sizeof(TG)) % 16 == 0)) &&
+                      (a.ld_y * sizeof(TY)) % 16 == 0;
+  if (ALIGNED && pieces && T > 2 * sms && a.d <= 8192)
+    return fours <= 256    ? launch_norm_gate_rows<TY, TG, OUT, 2, 128>(a, T, sms, err, st)
+           : fours <= 640  ? launch_norm_gate_rows<TY, TG, OUT, 2, 320>(a, T, sms, err, st)
+           : fours <= 1280 ? launch_norm_gate_rows<TY, TG, OUT, 2, 640>(a, T, sms, err, st)
+                           : launch_norm_gate_rows<TY, TG, OUT, 2, 1024>(a, T, sms, err, st);
 #define NORM_GATE_LAUNCH(FOURS, LONG, THREADS) return qv_launch(norm_gate_kernel<TY, TG, OUT, FOURS, ALIGNED, LONG>, dim3(T), dim3(THREADS), 0, st, a)
   if (fours > 2048) NORM_GATE_LAUNCH(1, true, 1024);
-  if (T <= 296 && fours <= 1024) NORM_GATE_LAUNCH(1, false, (fours + 31) / 32 * 32);
-  if (fours <= 512) NORM_GATE_LAUNCH(2, false, (fours + 63) / 64 * 32);
+  if (T <= 2 * sms && fours <= 1024) NORM_GATE_LAUNCH(1, false, (fours + 31) / 32 * 32);
   NORM_GATE_LAUNCH(4, false, (fours + 127) / 128 * 32);
 #undef NORM_GATE_LAUNCH
 }
@@ -216,7 +370,7 @@ int launch_norm_gate(const NormGateArgs& a, int T, cudaStream_t st) {
 // 2 8-bit rows with out_scale.
 extern "C" int qv_norm_gate_add(const float* stream, float* into, const void* y, long long ld_y, int y_dt, const float* w_post, float eps_post,
                                 const void* gate, long long ld_gate, int gate_dt, const float* gate_bias, const float* scale, const float* w_next,
-                                float eps_next, void* out, long long ld_out, int out_kind, float* out_scale, int T, int d, void* cuda_stream) {
+                                float eps_next, void* out, long long ld_out, int out_kind, float* out_scale, int T, int d, int* err, void* cuda_stream) {
   if (T <= 0 || d <= 0) return 0;
   if ((out_kind == 2) != (out_scale != nullptr) || out_kind < 0 || out_kind > 2) return QV_ERR_UNSUPPORTED;
   NormGateArgs a;
@@ -230,13 +384,15 @@ extern "C" int qv_norm_gate_add(const float* stream, float* into, const void* y,
   const bool aligned = d % 4 == 0 && (wide & 15) == 0 && ((uintptr_t)y & (4 * ysz - 1)) == 0 && ld_y % 4 == 0 && ((uintptr_t)gate & (4 * gsz - 1)) == 0 &&
                        ld_gate % 4 == 0 && ((uintptr_t)out & (4 * osz - 1)) == 0 && ld_out % 4 == 0;
   if (out_kind == 2 && (((uintptr_t)out & 3) || (ld_out & 3))) return QV_ERR_UNSUPPORTED;
-#define NORM_GATE_AS(TY, TG, OUT) return aligned ? launch_norm_gate<TY, TG, OUT, true>(a, T, st) : launch_norm_gate<TY, TG, OUT, false>(a, T, st)
+#define NORM_GATE_AS(TY, TG, OUT) return aligned ? launch_norm_gate<TY, TG, OUT, true>(a, T, err, st) : launch_norm_gate<TY, TG, OUT, false>(a, T, err, st)
 #define NORM_GATE(TY, TG)                        \
   do {                                           \
     if (out_kind == 0) NORM_GATE_AS(TY, TG, 0);  \
     if (out_kind == 1) NORM_GATE_AS(TY, TG, 1);  \
     NORM_GATE_AS(TY, TG, 2);                     \
   } while (0)
+  if (y_dt == QV_DT_F32 && !gate) NORM_GATE(float, NoGate);
+  if (y_dt == QV_DT_BF16 && !gate) NORM_GATE(bf16, NoGate);
   if (y_dt == QV_DT_F32 && gate_dt == QV_DT_F32) NORM_GATE(float, float);
   if (y_dt == QV_DT_F32 && gate_dt == QV_DT_BF16) NORM_GATE(float, bf16);
   if (y_dt == QV_DT_BF16 && gate_dt == QV_DT_F32) NORM_GATE(bf16, float);

@@ -133,7 +133,7 @@ _ARGTYPES = {
     "qv_pack_int8": [_V, _V, _L, _I, _I, _I, _V],
     "qv_gemm_int8": [_V, _L, _I, _V, _L, _V, _V, _V, _I, _I, _I, _I, _V, _I, _I, _I, _F, _F, _V, _V],
     "qv_linear_int8": [_V, _L, _I, _V, _L, _I, _V, _L, _V, _V, _V, _I, _I, _I, _I, _F, _F, _V, _V],
-    "qv_norm_gate_add": [_V, _V, _V, _L, _I, _V, _F, _V, _L, _I, _V, _V, _V, _F, _V, _L, _I, _V, _I, _I, _V],
+    "qv_norm_gate_add": [_V, _V, _V, _L, _I, _V, _F, _V, _L, _I, _V, _V, _V, _F, _V, _L, _I, _V, _I, _I, _V, _V],
     "qv_argmax": [_V, _V, _I, _I, _L, _V],
     "qv_argmax_ctas": [_I, _I],
     "qv_sample": [_V, _V, _I, _I, _L, _V, _V, _V, _V, _V, _V, _I, _V, _V, _V, _V],
@@ -2015,7 +2015,7 @@ def norm_gate_add(residual, y=None, post_weight=None, post_eps: float = 0.0, gat
         return
     rc = _lib("norm_gate").qv_norm_gate_add(
         residual.data_ptr(), into.data_ptr(), _ptr(y), ld_y, y_dt, _ptr(post_weight), post_eps, _ptr(gate), ld_gate, gate_dt, _ptr(gate_bias), _ptr(scale),
-        _ptr(next_weight), next_eps, _ptr(o), ld_out, out_kind, out.scale.data_ptr() if rows8 else None, T, d, _stream())
+        _ptr(next_weight), next_eps, _ptr(o), ld_out, out_kind, out.scale.data_ptr() if rows8 else None, T, d, _err_word(dev), _stream())
     _check(rc, "norm_gate_add")
 
 
