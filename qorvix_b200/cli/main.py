@@ -2,8 +2,8 @@
 word; flags are `--flag value`, core/src/main.cpp:269-303):
 
   qorvix generate <model_dir> --tokens 1,2,3 | --random-prompt N  [--max N] [--temp T] [--top-k K]
-                  [--top-p P] [--seed S] [--dtype bfloat16|float32]
-  qorvix bench <model_dir> [--prompt N] [--gen N] [--warmup N] [--runs N] [--batch B] [--json]
+                  [--top-p P] [--seed S] [--dtype bfloat16|float32] [--weights stored|int8]
+  qorvix bench <model_dir> [--prompt N] [--gen N] [--warmup N] [--runs N] [--batch B] [--weights stored|int8] [--json]
   qorvix model-info <model_dir>
   qorvix gpu-check <model_dir> [--tokens ...]      engine float32 and bfloat16 against the plain C++ CPU model
   qorvix random-model <out_dir> --config <config.json> [--seed S] [--dtype bfloat16|float32]
@@ -54,7 +54,7 @@ def cmd_generate(args) -> int:
     from ..sampling import SamplingParams
     if len(args) < 2:
         print("usage: qorvix generate <model_dir> --tokens 1,2,3 | --random-prompt N [--max N] [--temp T] "
-              "[--top-k K] [--top-p P] [--seed S] [--dtype bfloat16|float32]", file=sys.stderr)
+              "[--top-k K] [--top-p P] [--seed S] [--dtype bfloat16|float32] [--weights stored|int8]", file=sys.stderr)
         return 1
     model = args[1]
     cfg = load_config(model)
@@ -71,7 +71,7 @@ def cmd_generate(args) -> int:
     t0 = time.perf_counter()
     max_seq = len(prompt) + sp.max_new_tokens + 4            # as the reference sizes its engine (main.cpp:566)
     llm = LLM(model, dtype=flag_value(args, "--dtype", "bfloat16"), max_tokens=max_seq + 64,
-              max_concurrent=1, max_model_len=max_seq)
+              max_concurrent=1, max_model_len=max_seq, weights=flag_value(args, "--weights", "stored"))
     load_s = time.perf_counter() - t0
     print(" ".join(map(str, prompt)), flush=True)
     res = llm.generate([prompt], sp, on_token=lambda rid, tok: print(tok, end=" ", flush=True))[0]
@@ -170,13 +170,14 @@ def cmd_bench(args) -> int:
     from ..config import load_config
     from ..engine import ModelRunner, StepEntry
     if len(args) < 2:
-        print("usage: qorvix bench <model_dir> [--prompt N] [--gen N] [--warmup N] [--runs N] [--batch B] [--dtype D] [--json]", file=sys.stderr)
+        print("usage: qorvix bench <model_dir> [--prompt N] [--gen N] [--warmup N] [--runs N] [--batch B] [--dtype D] [--weights W] [--json]", file=sys.stderr)
         return 1
     P, G = int(flag_value(args, "--prompt", 64)), int(flag_value(args, "--gen", 128))
     warm, runs, B = int(flag_value(args, "--warmup", 1)), int(flag_value(args, "--runs", 3)), int(flag_value(args, "--batch", 1))
     cfg = load_config(args[1])
     t0 = time.perf_counter()
-    r = ModelRunner(args[1], dtype=flag_value(args, "--dtype", "bfloat16"), max_tokens=B * (P + G + 64), max_requests=B)
+    r = ModelRunner(args[1], dtype=flag_value(args, "--dtype", "bfloat16"), max_tokens=B * (P + G + 64), max_requests=B,
+                    weights=flag_value(args, "--weights", "stored"))
     load_s = time.perf_counter() - t0
     stream = [(i * 2654435761) % cfg.vocab_size for i in range(P + G)]      # the reference's token stream (benchmark.hpp:75)
     pre, dec = [], []

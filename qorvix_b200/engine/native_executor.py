@@ -109,6 +109,8 @@ class NativeExecutor:
             if type(b.mixer_norm) is not RMSNorm or type(b.ffn_norm) is not RMSNorm or type(b.mixer.position) is not RotaryEmbedding:
                 return None
             m, f = b.mixer, b.feed_forward
+            if any(lin.int8 is not None for lin in (m.qkv_proj, m.o_proj, f.gate_up, f.down)):
+                return None                        # it knows matrices as stored only
             if m.spec.kv_from is not None or b.mixer_norm.eps != model.final_norm.eps or b.ffn_norm.eps != model.final_norm.eps:
                 return None
             view = cache.layer_view(run)

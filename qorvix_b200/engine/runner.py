@@ -36,12 +36,21 @@ def parse_dtype(dtype) -> torch.dtype:
     return _DTYPES[str(dtype)]
 
 
+WEIGHTS = ("stored", "int8")
+
+
 class ModelRunner:
     def __init__(self, model_dir=None, *, config=None, tensors=None, dtype="bfloat16", max_tokens: int = 4096,
                  page_size: int = 16, max_requests: int = 8, max_model_len: Optional[int] = None,
-                 device="cuda", use_graphs: bool = True, max_graph_batch: int = 64):
+                 device="cuda", use_graphs: bool = True, max_graph_batch: int = 64, weights: str = "stored"):
         """model_dir: folder with config.json and model.safetensors; or config + tensors (a
-        mapping name -> tensor) for a model held in memory.  max_tokens sizes the page pool."""
+        mapping name -> tensor) for a model held in memory.  max_tokens sizes the page pool.
+        weights: "stored", or "int8" (bfloat16 only): the layers' large matrices are put into 8-bit integers with a scale for each
+        output channel when the model is loaded, and their products run over 8-bit rows with a scale for each token."""
+        if weights not in WEIGHTS:
+            raise ValueError(f"weights must be one of {', '.join(WEIGHTS)}, not {weights!r}")
+        if weights == "int8" and parse_dtype(dtype) != torch.bfloat16:
+            raise ValueError("weights in 8 bits go with dtype bfloat16")
         self.device = torch.device(device)
         _require_cuda(self.device)
         self.dtype = parse_dtype(dtype)
@@ -61,7 +70,7 @@ class ModelRunner:
         limit = self.spec.max_position if self.spec.max_position else pool_tokens
         self.max_model_len = int(max_model_len) if max_model_len else min(limit, pool_tokens)
         self.rt = Runtime(device=self.device, dtype=self.dtype, max_positions=self.max_model_len,
-                          page_size=self.page_size)
+                          page_size=self.page_size, weights=weights)
         if self.dtype == torch.bfloat16:
             ops.prepare_products(self.device)
         self.model = TextModel(self.spec, source, self.rt)

@@ -11,7 +11,7 @@ import torch
 
 from ..csrc import ops
 from ..parts.base import Runtime
-from ..parts.linear import Linear
+from ..parts.linear import Linear, int8_weights
 from ..parts.registry import build_part
 
 
@@ -26,7 +26,9 @@ class TextModel:
         else:                                      # an embedding part (more than one table, state of its own)
             self.embedder = build_part("embedding", spec.embedding, source, rt)
             self.embedding = self.embedder.weight
-        self.blocks = [build_part("block", _BlockView(layer), source, rt) for layer in spec.layers]
+        # in 8 bits where the runtime says so: the layers' matrices; the embedding and the head stay as stored
+        with int8_weights(rt.weights == "int8"):
+            self.blocks = [build_part("block", _BlockView(layer), source, rt) for layer in spec.layers]
         self.final_norm = build_part("norm", spec.final_norm, source, rt)
         self.lm_head = Linear(source.get(spec.lm_head)) if spec.lm_head is not None else Linear(self.embedding)
         self.order: List[int] = list(spec.order)

@@ -42,8 +42,12 @@ class Attention(Mixer):
 
     folds_norms = True             # forward() takes a PreNormed x, residual= and next_norm=
 
+    @property
+    def takes_int8_rows(self) -> bool:
+        return self.qkv_proj.int8 is not None
+
     def forward(self, x, ctx, cache, residual=None, next_norm=None):
-        """x: the normed rows [T, d], or a PreNormed (few tokens: the norm's scale is then applied to the
+        """x: the normed rows [T, d] (ops.Int8Rows too where takes_int8_rows), or a PreNormed (few tokens: the norm's scale is then applied to the
         projection's sums).  With residual and next_norm the output projection adds the output to the
         stream itself and the PreNormed input of next_norm is returned instead of the output."""
         H, Hkv, hd = self.H, self.Hkv, self.hd

@@ -11,6 +11,7 @@ FeedForward   forward(x[T,d], ctx) -> [T,d].
               the stream next>; it may then add its output to the stream itself and return a
               PreNormed for that norm (few tokens: the norm's two passes over the stream ride in the
               epilogues of the products around it).
+              One with takes_int8_rows = True also takes x as ops.Int8Rows (its products keep their matrices in 8 bits).
 Norm          add_norm(residual, delta, rows=None): residual (float32) += delta (delta may be None), returns
               the normed rows in the compute dtype; with rows (int32 row indices) only those rows of
               residual + delta are normed and the residual is left as it is.  The sum and the norm
@@ -19,6 +20,8 @@ Norm          add_norm(residual, delta, rows=None): residual (float32) += delta 
               folds_into_products = True and give size, eps and scale_weight() (w as float32): parts
               that fold norms then take its two passes over the stream into the epilogues of the
               products around it.  Nothing else about the norm is assumed.
+              A norm may offer add_norm_int8(residual, delta) -> ops.Int8Rows; a block that found all readers
+              of the norm's rows to take them in 8 bits sets int8_rows = True on it.
 Position      table() -> float32 [positions, rotary_dim/2, 2] of (cos, sin) if it is a rotation
               the attention kernels can fuse, else None; apply(qkv, ctx, H, Hkv, hd) rotates q and k
               in place for mixers that do not fuse it.
@@ -42,6 +45,7 @@ class Runtime:
     dtype: torch.dtype                 # compute dtype: torch.bfloat16 or torch.float32
     max_positions: int                 # rows of position tables
     page_size: int = 16
+    weights: str = "stored"            # "int8": the layers' large matrices in 8-bit integers, their products over 8-bit rows
 
     def empty(self, *shape, dtype=None) -> torch.Tensor:
         return torch.empty(shape, device=self.device, dtype=dtype or self.dtype)
@@ -108,6 +112,7 @@ class FeedForward:
 
 class Norm:
     folds_into_products = False        # True: see the module's header; needs size, eps, scale_weight()
+    int8_rows = False                  # set by the block that owns the norm: all readers of its rows take ops.Int8Rows
 
     def add_norm(self, residual, delta, rows=None):
         raise NotImplementedError

@@ -2,7 +2,7 @@
     x += mixer(norm(x));  x += feed_forward(norm(x))
 The residual stream is float32.  A block hands the feed-forward's output on as a pending
 delta, which the next norm adds in its own pass.  'post_norm' puts the norms on the parts' outputs instead, 'sandwich_norm'
-on both sides of a part; 'hyper' is 'pre_norm' over several residual streams."""
+on both sides of a part (with a gate and a scale on what it adds, where the layer names them); 'hyper' is 'pre_norm' over several residual streams."""
 from __future__ import annotations
 
 import torch
@@ -20,6 +20,8 @@ class PreNormBlock(Block):
         self.mixer = build_part("mixer", spec.mixer, source, rt)
         self.ffn_norm = build_part("norm", spec.ffn_norm, source, rt)
         self.feed_forward = build_part("feed_forward", spec.feed_forward, source, rt)
+        _mark_int8(self.mixer_norm, self.mixer)
+        _mark_int8(self.ffn_norm, self.feed_forward)
 
     def forward(self, residual, pending, ctx, cache):
         # Few tokens: a part that folds norms (folds_norms) is told which norm (one that folds into products) reads the stream
@@ -51,7 +53,7 @@ class PreNormBlock(Block):
             return pending.rows
         if isinstance(pending, PreNormed) and pending.norm is norm and getattr(part, "folds_norms", False):
             return pending
-        return norm.add_norm(residual, pending)
+        return norm.add_norm_int8(residual, pending) if getattr(norm, "int8_rows", False) else norm.add_norm(residual, pending)
 
     def first_norm(self):
         """The norm this block reads the stream with first (what the block ahead may prepare for)."""
@@ -63,6 +65,12 @@ class PreNormBlock(Block):
 def _folds(norm) -> bool:
     """Whether a norm lets the products around it take over its passes (see parts/base.py)."""
     return norm is not None and getattr(norm, "folds_into_products", False)
+
+
+def _mark_int8(norm, *readers) -> None:
+    """Notes on a norm that everything that reads its rows takes them in 8 bits."""
+    if norm is not None and hasattr(norm, "add_norm_int8"):
+        norm.int8_rows = all(getattr(r, "takes_int8_rows", False) for r in readers if r is not None)
 
 
 class ParallelBlock(Block):
@@ -225,7 +233,8 @@ class PostNormBlock(Block):
 
 
 class SandwichNormBlock(Block):
-    """x += post_a(mixer(norm_a(x)));  x += post_b(feed_forward(norm_b(x))).  The pass that adds a part's normed output to the float32
+    """x += post_a(mixer(norm_a(x)));  x += post_b(feed_forward(norm_b(x))).  Where the layer names a gate or a scale, what is added is
+    scale * sigmoid(W h + b) * post(part(h)), h the part's input (W [width, width], b its ".b"; scale a number per feature).  The pass that adds a part's normed output to the float32
     stream also applies the norm of the part after it (of this block, or the one the next block starts with), so the stream is
     read and written once a part; the next block finds its first part's input as a ReadyNormed."""
 
@@ -235,6 +244,10 @@ class SandwichNormBlock(Block):
         self.feed_forward = build_part("feed_forward", spec.feed_forward, source, rt)
         self.mixer_norm, self.mixer_post = self._norms(self.mixer, spec.mixer_norm, spec.mixer_post_norm, source, rt)
         self.ffn_norm, self.ffn_post = self._norms(self.feed_forward, spec.ffn_norm, spec.ffn_post_norm, source, rt)
+        self.mixer_extra = self._extra(self.mixer, self.mixer_post, getattr(spec, "mixer_gate", None), getattr(spec, "mixer_scale", None), source)
+        self.ffn_extra = self._extra(self.feed_forward, self.ffn_post, getattr(spec, "ffn_gate", None), getattr(spec, "ffn_scale", None), source)
+        _mark_int8(self.mixer_norm, self.mixer, self.mixer_extra[0])
+        _mark_int8(self.ffn_norm, self.feed_forward, self.ffn_extra[0])
 
     @staticmethod
     def _norms(part, before, after, source, rt):
@@ -245,29 +258,51 @@ class SandwichNormBlock(Block):
             raise ValueError("a sandwich-norm block needs norms that can be added to the stream (add_normed)")
         return pre, post
 
+    @staticmethod
+    def _extra(part, post, gate, scale, source):
+        """(gate product, its bias, scale) of a part, each None where the layer names none."""
+        if part is None or (gate is None and scale is None):
+            return None, None, None
+        if not _folds(post):
+            raise ValueError("a sandwich-norm block with a gate or a scale needs an RMS norm behind the part")
+        return (Linear(source.get(gate)) if gate is not None else None, source.get(gate + ".b", dtype=torch.float32) if gate is not None else None,
+                source.get(scale, dtype=torch.float32).contiguous() if scale is not None else None)
+
     def _input(self, norm, residual, pending):
         if isinstance(pending, ReadyNormed) and pending.norm is norm:
             return pending.rows
-        return norm.add_norm(residual, pending)
+        return norm.add_norm_int8(residual, pending) if getattr(norm, "int8_rows", False) else norm.add_norm(residual, pending)
 
-    def _add(self, post, residual, y, nxt):
+    def _add(self, post, residual, y, nxt, h, extra):
         """The stream takes the normed output; `nxt` (the norm that reads the stream next, or None) is applied in the same pass
         where it is an RMS norm over the stream."""
-        if not _folds(nxt) or nxt.size != residual.shape[1]:
-            post.add_normed(residual, y)
-            return None
-        rows = torch.empty(residual.shape, device=residual.device, dtype=self.rt.dtype)
-        post.add_normed(residual, y, cast=rows, next_norm=nxt)
-        return ReadyNormed(norm=nxt, residual=residual, rows=rows)
+        gate, bias, scale = extra
+        joins = _folds(nxt) and nxt.size == residual.shape[1]
+        if gate is None and scale is None and not (joins and getattr(nxt, "int8_rows", False) and _folds(post)):
+            if not joins:
+                post.add_normed(residual, y)
+                return None
+            rows = torch.empty(residual.shape, device=residual.device, dtype=self.rt.dtype)
+            post.add_normed(residual, y, cast=rows, next_norm=nxt)
+            return ReadyNormed(norm=nxt, residual=residual, rows=rows)
+        rows = None
+        if joins:
+            rows = (ops.int8_rows(*residual.shape, residual.device) if getattr(nxt, "int8_rows", False)
+                    else torch.empty(residual.shape, device=residual.device, dtype=self.rt.dtype))
+        ops.norm_gate_add(residual, y, post_weight=post.scale_weight(), post_eps=post.eps, gate=gate(h, out_dtype=torch.float32) if gate is not None else None,
+                          gate_bias=bias, scale=scale, next_weight=nxt.scale_weight() if joins else None, next_eps=nxt.eps if joins else 0.0, out=rows)
+        return ReadyNormed(norm=nxt, residual=residual, rows=rows) if joins else None
 
     def forward(self, residual, pending, ctx, cache):
         after = getattr(ctx, "next_norm", None)
         if self.mixer is not None:
-            y = self.mixer.forward(self._input(self.mixer_norm, residual, pending), ctx, cache)
-            pending = self._add(self.mixer_post, residual, y, self.ffn_norm if self.feed_forward is not None else after)
+            h = self._input(self.mixer_norm, residual, pending)
+            y = self.mixer.forward(h, ctx, cache)
+            pending = self._add(self.mixer_post, residual, y, self.ffn_norm if self.feed_forward is not None else after, h, self.mixer_extra)
         if self.feed_forward is not None:
-            y = self.feed_forward.forward(self._input(self.ffn_norm, residual, pending), ctx)
-            pending = self._add(self.ffn_post, residual, y, after)
+            h = self._input(self.ffn_norm, residual, pending)
+            y = self.feed_forward.forward(h, ctx)
+            pending = self._add(self.ffn_post, residual, y, after, h, self.ffn_extra)
         return residual, pending
 
     def first_norm(self):

@@ -48,7 +48,7 @@ class LatentAttention(Mixer):
         # portions form every head's keys and values once: one product of the latents with both matrices
         self.kv_up = None
         if rt.dtype == torch.bfloat16 and self.k_up.dtype == torch.bfloat16 and (self.dn, self.dr, self.dv) == (128, 64, 128):
-            up = Linear(torch.cat([self.k_up, self.v_up], dim=0))
+            up = Linear(torch.cat([self.k_up, self.v_up], dim=0), as_stored=True)
             self.kv_up = (up.packed, up.out_features) if up.packed is not None else None
         self.o_proj = Linear(source.get(spec.o_proj))
         self.position = build_part("position", spec.position, source, rt)

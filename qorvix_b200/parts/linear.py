@@ -2,25 +2,59 @@
 weight's dtype and the shape: float32 weights run on the CUDA cores in true float32;
 bfloat16 weights run on the tensor-core kernels where the shape allows, else on the same
 CUDA-core kernel with float32 accumulation.  All of them are kernels of this package.
+
+Within `int8_weights()` bfloat16 matrices of INT8_LEAST entries and more are kept in 8-bit integers with a scale for each output
+channel; a product then puts its rows into 8 bits too, a scale each (ops.gemm_int8).
 """
 from __future__ import annotations
+
+import contextlib
+import contextvars
 
 import torch
 
 from ..csrc import ops
 from .base import PreNormed
 
+# Smaller matrices stay as they are stored: a megabyte of weights less is 0.2 us of a step, and putting the rows into 8 bits costs a launch.
+INT8_LEAST = 1 << 20
+
+_int8 = contextvars.ContextVar("int8_weights", default=False)
+
+
+@contextlib.contextmanager
+def int8_weights(on: bool = True):
+    """Linear layers (and routed experts) built inside keep their matrices in 8 bits."""
+    token = _int8.set(bool(on))
+    try:
+        yield
+    finally:
+        _int8.reset(token)
+
+
+def wants_int8(weight: torch.Tensor) -> bool:
+    """Whether a matrix [N, K], or matrices [E, N, K], built now go into 8 bits."""
+    return (_int8.get() and weight.is_cuda and weight.dtype == torch.bfloat16 and weight.shape[-2] * weight.shape[-1] >= INT8_LEAST
+            and weight.shape[-1] <= ops.INT8_MAX_K)
+
 
 class Linear:
-    def __init__(self, weight: torch.Tensor, keep_rows: bool = False):
+    int8 = None                        # ops.Int8Weight where the matrix is kept in 8 bits
+
+    def __init__(self, weight: torch.Tensor, keep_rows: bool = False, as_stored: bool = False):
+        """as_stored: never in 8 bits (the packed tiles are read by other kernels)."""
         assert weight.dim() == 2
         self.weight = weight.contiguous()
         self.out_features, self.in_features = weight.shape
+        self.packed = None
+        if not as_stored and wants_int8(self.weight):
+            self.int8 = ops.quantize_weight(self.weight)
+            self.weight = None
+            return
         # A bfloat16 matrix is stored as the 16 KB tiles the MMA consumes (128 rows x 64 k in its
         # swizzled shared-memory layout), which HBM and an SM's copy engine deliver faster than
         # rows; the rows are then dropped (keep_rows, or QORVIX_KEEP_ROWS=1, keeps them, for tests
         # that compare the two layouts).
-        self.packed = None
         if (self.weight.is_cuda and self.weight.dtype == torch.bfloat16 and self.in_features % 8 == 0
                 and ops.packed_weights_enabled()):
             try:
@@ -30,11 +64,19 @@ class Linear:
             if self.packed is not None and not (keep_rows or _keep_rows()):
                 self.weight = None
 
+    @property
+    def takes_int8_rows(self) -> bool:
+        return self.int8 is not None
+
     def forward(self, x: torch.Tensor, out: torch.Tensor = None, out_dtype: torch.dtype = None) -> torch.Tensor:
+        """x: rows, or, where the matrix is kept in 8 bits, ops.Int8Rows too (out or out_dtype is then given)."""
         M = x.shape[0]
         if out is None:
             out = torch.empty((M, self.out_features), device=x.device, dtype=out_dtype or x.dtype)
         if M == 0:
+            return out
+        if self.int8 is not None:
+            ops.gemm_int8(out, x, self.int8)
             return out
         ops.gemm(out, x, self.weight, self.packed, self.out_features, settled=True)
         return out

@@ -42,8 +42,12 @@ class SwiGLU(FeedForward):
 
     folds_norms = True             # forward() takes a PreNormed x, residual= and next_norm=
 
+    @property
+    def takes_int8_rows(self) -> bool:
+        return self.gate_up.int8 is not None
+
     def forward(self, x, ctx, residual=None, next_norm=None):
-        """x: the normed rows [T, d], or a PreNormed (few tokens: the norm's scale is then applied to the
+        """x: the normed rows [T, d] (ops.Int8Rows too where takes_int8_rows), or a PreNormed (few tokens: the norm's scale is then applied to the
         gate/up sums before the activation).  With residual and next_norm the down projection adds the
         output to the stream itself and the PreNormed input of next_norm is returned instead."""
         act = None
@@ -53,7 +57,9 @@ class SwiGLU(FeedForward):
                 act, x = None, x.materialise()
         if act is None:
             act = torch.empty((x.shape[0], self.f), device=x.device, dtype=self.rt.dtype)
-            if self.interleaved:
+            if self.interleaved and self.gate_up.int8 is not None:
+                ops.gemm_int8_glu(act, x, self.gate_up.int8, self.act, limit=self.limit, slope=self.slope)
+            elif self.interleaved:
                 ops.gemm_swiglu(act, x, self.gate_up.weight, self.gate_up.packed, self.gate_up.out_features, act=self.act,
                                 limit=self.limit, slope=self.slope, settled=True)
             else:
@@ -84,7 +90,11 @@ class ActMLP(FeedForward):
 
     def forward(self, x, ctx, with_bias: bool = True):
         act = torch.empty((x.shape[0], self.up.out_features), device=x.device, dtype=self.rt.dtype)
-        ops.gemm_act(act, x, self.up.weight, self.up.packed, self.up.out_features, self.act, self.up_bias)
+        if self.up.int8 is not None:
+            self.up(x, out=act)
+            ops.activation(act, act, self.act, bias=self.up_bias)
+        else:
+            ops.gemm_act(act, x, self.up.weight, self.up.packed, self.up.out_features, self.act, self.up_bias)
         if self.output_bias is None or not with_bias:
             return self.down(act, out_dtype=self.rt.dtype)
         y = self.down(act, out_dtype=torch.float32)

@@ -9,6 +9,7 @@ import torch
 from ..csrc import ops
 from .base import FeedForward
 from .mlp import GLU_ACTIVATIONS
+from .linear import wants_int8
 from .registry import build_part, register_part
 
 
@@ -26,7 +27,15 @@ class RoutedFeedForward(FeedForward):
         # (the rows are then dropped)
         self.tensor_cores = (rt.dtype == torch.bfloat16 and self.w_gate.dtype == torch.bfloat16 and spec.hidden_size % 8 == 0
                              and spec.expert_ff % 8 == 0)
-        if self.tensor_cores:
+        # in 8 bits: gate and up rows alternate in groups of 16, as the product's epilogue takes them
+        self.int8 = None
+        if self.tensor_cores and spec.expert_ff % 16 == 0 and wants_int8(self.w_gate) and wants_int8(self.w_down):
+            E, ff, d = self.w_gate.shape
+            both = torch.stack([self.w_gate.view(E, ff // 16, 16, d), self.w_up.view(E, ff // 16, 16, d)], dim=2).view(E, 2 * ff, d)
+            self.w_gate = self.w_up = None
+            self.int8 = (ops.quantize_weight(both), ops.quantize_weight(self.w_down))
+            self.w_down = both = None
+        elif self.tensor_cores:
             self.w_gate, self.w_up, self.w_down = (ops.moe_pack_experts(w) for w in (self.w_gate, self.w_up, self.w_down))
         self.shared = build_part("feed_forward", spec.shared, source, rt)
         gated = spec.shared is not None and spec.shared_gate is not None
@@ -50,14 +59,22 @@ class RoutedFeedForward(FeedForward):
         gate = torch.empty(T, device=dev, dtype=torch.float32) if self.shared_gate is not None else None
         ops.moe_route(top_idx, top_w, gate, x, self.router, self.shared_gate, **self.routing)
         tc = self.tensor_cores
-        tile_rows = ops.moe_tile_rows(tc, T, R, s.experts)
+        tile_rows = ops.moe_int8_tile_rows(R, s.experts) if self.int8 is not None else ops.moe_tile_rows(tc, T, R, s.experts)
         n_tiles = 3 * ops.moe_max_tiles(R, s.experts, tile_rows)
         ints = torch.empty(3 * R + n_tiles, device=dev, dtype=torch.int32)
         row_token, slot_row, scratch, tiles = ints.split_with_sizes((R, R, R, n_tiles))
         ops.moe_group(row_token, slot_row, tiles, top_idx, scratch, s.experts, tile_rows)
         act = torch.empty((R, s.expert_ff), device=dev, dtype=x.dtype)
         y = torch.empty((R, d), device=dev, dtype=torch.float32)
-        if tc:
+        if self.int8 is not None:
+            up, down = self.int8
+            rows = ops.int8_rows(R, d, dev)
+            ops.quantize_rows(rows, x, row_idx=row_token)
+            ops.moe_experts_int8(True, act, rows, up, tiles, tile_rows=tile_rows, **self.glu)
+            rows = ops.int8_rows(R, s.expert_ff, dev)
+            ops.quantize_rows(rows, act)
+            ops.moe_experts_int8(False, y, rows, down, tiles, tile_rows=tile_rows)
+        elif tc:
             ops.moe_experts_tc(True, act, x, self.w_gate, self.w_up, row_token, tiles, tile_rows=tile_rows, room=y, **self.glu)
             ops.moe_experts_tc(False, y, act, self.w_down, None, row_token, tiles, tile_rows=tile_rows)
         else:

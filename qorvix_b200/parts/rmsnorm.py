@@ -38,6 +38,14 @@ class RMSNorm(Norm):
         return out
 
 
+    def add_norm_int8(self, residual, delta):
+        """As add_norm, with the rows in 8 bits (those of the bfloat16 rows) for the products that read them."""
+        if isinstance(delta, PreNormed):
+            delta = None                    # the product is in the stream already
+        out = ops.int8_rows(residual.shape[0], self.size, residual.device)
+        ops.norm_gate_add(residual, delta, next_weight=self.weight, next_eps=self.eps, out=out)
+        return out
+
     def add_normed(self, residual, y, cast=None, next_norm=None):
         """residual (float32) += rmsnorm(y) * weight: the norm on a sublayer's output.  `cast`, if given, receives the new
         stream in the compute type, with next_norm (one that declares folds_into_products) already normed by it."""

@@ -789,7 +789,8 @@ class LayerSpec:
     mixer_gate / ffn_gate name W [width, width], the bias is name + ".b".
     'post_norm': x += mixer_norm(mixer(x)); x += ffn_norm(feed_forward(x)): the parts read the stream itself and the norms
     sit on their outputs.
-    'sandwich_norm': x += mixer_post_norm(mixer(mixer_norm(x))); x += ffn_post_norm(feed_forward(ffn_norm(x))).
+    'sandwich_norm': x += mixer_post_norm(mixer(mixer_norm(x))); x += ffn_post_norm(feed_forward(ffn_norm(x))); with mixer_gate / ffn_gate and
+    mixer_scale / ffn_scale each sum is multiplied by sigmoid(W h + b), h being the part's input, and by the scale.
     'hyper': the pre-norm order on several residual streams, each part tied to them by mixer_link / ffn_link (StreamLinkSpec)."""
     mixer: object
     feed_forward: object
