@@ -13,6 +13,7 @@
 #include "int8_rows.cuh"
 #include "per_device.h"
 #include "tc_common.cuh"
+#include <type_traits>
 
 #define QK 128                        // k entries of a stage: 128 bytes, one swizzle span
 #define W_TILE_BYTES (BM * QK)
@@ -45,6 +46,9 @@ struct Int8Args {
   int N, K;
   int splits, kb_per_split;           // few rows: CTAs that share a block of channels, and the k blocks of each
   int mine_shift;                     // and, as a power of two, the columns of which each adds up the sums
+  const void* x;                      // few rows that the kernel itself puts into 8 bits: the rows, their stride, whether pieces lie on 16 bytes
+  long long ld_x;
+  int aligned;
   GluAct glu;
 };
 
@@ -302,24 +306,57 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
   }
 }
 
+// ---------------------------------------------------------------- pieces of a row: 16 bytes of it
+template <typename T> struct Piece { static constexpr int N = 16 / (int)sizeof(T); };
+template <typename T, bool ALIGNED> __device__ __forceinline__ uint4 load_piece(const T* x, int k, int K) {
+  constexpr int N = Piece<T>::N;
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (ALIGNED && k + N <= K) return *(const uint4*)(x + k);
+  T* e = (T*)&v;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (k + i < K) e[i] = x[k + i];
+  return v;
+}
+// The largest magnitude so far, of bfloat16 a pair of them (their bits are ordered as float32's are).
+__device__ __forceinline__ uint32_t larger(uint32_t top, const uint4& v, const float*) {
+  constexpr uint32_t M = 0x7fffffffu;
+  return max(max(top, max(v.x & M, v.y & M)), max(v.z & M, v.w & M));
+}
+__device__ __forceinline__ uint32_t larger(uint32_t top, const uint4& v, const bf16*) {
+  constexpr uint32_t M = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(top, __vmaxu2(v.x & M, v.y & M)), __vmaxu2(v.z & M, v.w & M));
+}
+__device__ __forceinline__ uint32_t top_bits(uint32_t top, const float*) { return top; }
+__device__ __forceinline__ uint32_t top_bits(uint32_t top, const bf16*) { return max(top << 16, top & 0xffff0000u); }
+
 // ---------------------------------------------------------------- few rows
 // A step of few tokens is bound by the matrix' bytes, so that all SMs have to ask for weights at once, and from the start: a block of 128
 // channels is shared along k by the CTAs of a cluster (grid z), each with a ring of its own, and the first weights are asked for before the
 // wait for the kernel ahead (a packed matrix lies still: qv_pack_int8 lets no kernel start before its end).  The CTAs hand their int32 sums
-// to one another through distributed shared memory: CTA s adds up columns s, s + splits, ... of all of them, scales and stores these; whole
+// to one another through distributed shared memory: each adds up a share of the columns of all of them, scales and stores these; whole
 // sums have no order, so splits change no bit.
-template <bool GLU, typename TO, int BN, int STAGES>
-__global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ CUtensorMap map_x, const Int8Args p) {
+// TX void: the rows are in 8 bits already and come with the weights.  Else they are float32 or bfloat16 and every CTA puts them into 8 bits itself,
+// while its first weights are on their way: eight warps look for the largest entry of every row, then round the CTA's share of k into shared
+// memory.  That is a launch less, and all of it behind the weights' latency, as long as the rows are few and short (see rows_inside).
+#define FEW_QUANTIZERS 256
+template <bool GLU, typename TO, typename TX, int BN, int STAGES>
+__global__ void __launch_bounds__(std::is_void<TX>::value ? 192 : 64 + FEW_QUANTIZERS) int8_few_kernel(const __grid_constant__ CUtensorMap map_x, const Int8Args p) {
   extern __shared__ uint8_t smem_raw[];
-  constexpr int STAGE_BYTES = W_TILE_BYTES + BN * QK;
+  constexpr bool INSIDE = !std::is_void<TX>::value;
+  constexpr int STAGE_BYTES = W_TILE_BYTES + (INSIDE ? 0 : BN * QK);
   constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
   uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = (uint64_t*)(ring + STAGES * STAGE_BYTES);
+  uint8_t* rows8 = ring + STAGES * STAGE_BYTES;                // INSIDE: [k blocks of this CTA][BN rows][128], as the products read them
+  uint8_t* behind = rows8 + (INSIDE ? p.kb_per_split * BN * QK : 0);
+  uint64_t* full = (uint64_t*)behind;
   uint64_t* empty = full + STAGES;
   uint64_t* accum = empty + STAGES;
-  uint32_t* tmem_slot = (uint32_t*)(accum + 1);
+  uint64_t* rows_there = accum + 1;
+  uint32_t* tmem_slot = (uint32_t*)(rows_there + 1);
   __shared__ __align__(16) float xs[BN];                       // the rows' scales
-  int* sums = (int*)(ring + STAGES * STAGE_BYTES + 256);       // [splits][columns of this CTA / 4][128 channels][4]: what the cluster hands this CTA
+  __shared__ uint32_t tops[BN];                                // INSIDE: the rows' largest magnitudes
+  int* sums = (int*)(behind + 256);                            // [splits][columns of this CTA / 4][128 channels][4]: what the cluster hands this CTA
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int KT = (p.K + QK - 1) / QK;
   const int split = blockIdx.z, kb0 = split * p.kb_per_split;
@@ -328,6 +365,7 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     mbar_init(accum, 1);
+    mbar_init(rows_there, FEW_QUANTIZERS);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -352,10 +390,12 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
         bulk_load_1d(ring + kb * STAGE_BYTES, w + (size_t)kb * W_TILE_BYTES, &full[kb], W_TILE_BYTES);
       }
     __syncwarp();
-    pdl_wait();
-    if (leader)
-      for (int kb = 0; kb < pre; ++kb) tma_load_2d(ring + kb * STAGE_BYTES + W_TILE_BYTES, &map_x, &full[kb], (kb0 + kb) * QK, row0);
-    __syncwarp();
+    if (!INSIDE) {
+      pdl_wait();
+      if (leader)
+        for (int kb = 0; kb < pre; ++kb) tma_load_2d(ring + kb * STAGE_BYTES + W_TILE_BYTES, &map_x, &full[kb], (kb0 + kb) * QK, row0);
+      __syncwarp();
+    }
     int kb = pre;
     for (; kb < num_kb; ++kb) {
       const int s = kb % STAGES;
@@ -364,7 +404,7 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
         uint8_t* dst = ring + s * STAGE_BYTES;
         mbar_expect_tx(&full[s], STAGE_BYTES);
         bulk_load_1d(dst, w + (size_t)kb * W_TILE_BYTES, &full[s], W_TILE_BYTES);
-        tma_load_2d(dst + W_TILE_BYTES, &map_x, &full[s], (kb0 + kb) * QK, row0);
+        if (!INSIDE) tma_load_2d(dst + W_TILE_BYTES, &map_x, &full[s], (kb0 + kb) * QK, row0);
       }
       __syncwarp();
     }
@@ -373,12 +413,13 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
   } else if (warp == 1) {
     const bool leader = elect_one();
     const uint32_t idesc = umma_idesc_i8(BM, BN);
-    for (int kb = 0; kb < num_kb; ++kb) {
+    const bool there = !INSIDE || mbar_wait(rows_there, 0, p.err, 66);
+    for (int kb = 0; there && kb < num_kb; ++kb) {
       const int s = kb % STAGES;
       if (!mbar_wait(&full[s], (kb / STAGES) & 1, p.err, 62)) break;
       tc_fence_after();
-      const uint32_t a_addr = smem_u32(ring + s * STAGE_BYTES);
-      const uint64_t da = umma_desc(a_addr), db = umma_desc(a_addr + W_TILE_BYTES);
+      const uint32_t a_addr = smem_u32(ring + s * STAGE_BYTES), b_addr = INSIDE ? smem_u32(rows8 + kb * BN * QK) : a_addr + W_TILE_BYTES;
+      const uint64_t da = umma_desc(a_addr), db = umma_desc(b_addr);
       if (leader) {
 #pragma unroll
         for (int kk = 0; kk < QK / 32; ++kk) umma_i8(tmem_base, da + 2 * kk, db + 2 * kk, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
@@ -391,7 +432,8 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
   }
   const int q = warp & 3, ch0 = blockIdx.x * BM + q * 32;
   const int feat = GLU ? (ch0 >> 1) + (lane & 15) : ch0 + lane;
-  const bool there = warp >= 2 && (GLU ? 2 * feat < p.N : feat < p.N);
+  const bool stores = warp >= 2 && warp < 6;         // the epilogue's warps
+  const bool there = stores && (GLU ? 2 * feat < p.N : feat < p.N);
   TO* out = (TO*)p.out + (size_t)row0 * p.ld_out + feat;
   float ws = 0.f;
   // the scaled sums of columns c, c + 1, ... to the output: all lanes of an epilogue warp are here
@@ -418,17 +460,64 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
   };
   bool ok = true;
   if (warp >= 2) {
-    pdl_wait();                                      // the rows' scales are the kernel's ahead, and the output may still be in its use
-    if (ch0 + lane < p.N) ws = p.w_scale[ch0 + lane];
+    pdl_wait();                                      // the rows (or their scales) are the kernel's ahead, and the output may still be in its use
     const int te = threadIdx.x - 64;
-    if (te < BN) xs[te] = te < rows ? p.x_scale[row0 + te] : 0.f;
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    ok = __all_sync(0xffffffffu, mbar_wait(accum, 0, p.err, 63));
-    tc_fence_after();
+    if constexpr (INSIDE) {
+      constexpr int N = Piece<TX>::N;
+      const TX* x = (const TX*)p.x + (size_t)row0 * p.ld_x;
+      if (te < BN) tops[te] = 0u;
+      asm volatile("bar.sync 2, %0;" ::"n"(FEW_QUANTIZERS) : "memory");
+      const int per_row = rows < FEW_QUANTIZERS / 32 ? FEW_QUANTIZERS / 32 / rows : 1;         // warps that share a row
+      const int pieces = (p.K + N - 1) / N, share = (pieces + per_row - 1) / per_row;
+      for (int task = te >> 5; task < rows * per_row; task += FEW_QUANTIZERS / 32) {
+        const int r = task / per_row, from = (task - r * per_row) * share, to = from + share < pieces ? from + share : pieces;
+        const TX* xr = x + (size_t)r * p.ld_x;
+        uint32_t top = 0;
+        for (int i = from + lane; i < to; i += 256) {
+          uint4 v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            v[u] = i + 32 * u >= to ? make_uint4(0u, 0u, 0u, 0u) : p.aligned ? load_piece<TX, true>(xr, (i + 32 * u) * N, p.K) : load_piece<TX, false>(xr, (i + 32 * u) * N, p.K);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) top = larger(top, v[u], xr);
+        }
+        top = __reduce_max_sync(0xffffffffu, top_bits(top, xr));
+        if (lane == 0) atomicMax(&tops[r], top);
+      }
+      asm volatile("bar.sync 2, %0;" ::"n"(FEW_QUANTIZERS) : "memory");
+      for (int i = te; i < rows * num_kb * 8; i += FEW_QUANTIZERS) {                           // 16 entries each
+        const int r = i / (num_kb * 8), c = i - r * (num_kb * 8), k = (kb0 + (c >> 3)) * QK + (c & 7) * 16;
+        const TX* xr = x + (size_t)r * p.ld_x;
+        const Int8Scale s = int8_scale(__uint_as_float(tops[r]));
+        uint32_t w[4];
+#pragma unroll
+        for (int u = 0; u < 16 / N; ++u) {
+          const uint4 v = p.aligned ? load_piece<TX, true>(xr, k + u * N, p.K) : load_piece<TX, false>(xr, k + u * N, p.K);
+          const TX* e = (const TX*)&v;
+          float f[N];
+#pragma unroll
+          for (int m = 0; m < N; ++m) f[m] = to_f(e[m]);
+          uint32_t part[N / 4];
+          int8_pack<sizeof(TX) == 2, N>(f, s, part);
+#pragma unroll
+          for (int m = 0; m < N / 4; ++m) w[u * (N / 4) + m] = part[m];
+        }
+        *(uint4*)(rows8 + (c >> 3) * BN * QK + r * QK + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the products read them
+      mbar_arrive(rows_there);
+    }
+    if (stores) {
+      if (ch0 + lane < p.N) ws = p.w_scale[ch0 + lane];
+      if (te < BN) xs[te] = te >= rows ? 0.f : INSIDE ? int8_step(__uint_as_float(tops[te])) : p.x_scale[row0 + te];
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      ok = __all_sync(0xffffffffu, mbar_wait(accum, 0, p.err, 63));
+      tc_fence_after();
+    }
   }
   const int shift = p.mine_shift, mine = 1 << shift;           // columns a CTA adds up: 4 or more
   if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-  if (warp >= 2 && ok) {
+  if (stores && ok) {
     const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
     const uint32_t to = smem_u32(sums) + (uint32_t)(((split << (shift - 2)) * BM + q * 32 + lane) * 16);
 #pragma unroll 1
@@ -455,7 +544,7 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
   if (p.splits > 1) {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-    if (warp >= 2 && ok) {
+    if (stores && ok) {
       const int4* part = (const int4*)sums + q * 32 + lane;
       for (int i = 0; i < mine; i += 4) {
         const int c = (split << shift) + i;
@@ -482,29 +571,6 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ C
 // rounding: VECS pieces of 16 bytes a thread, all asked for at once.  A row has a warp (no barrier between its two halves, so that the SM's
 // other rows go on: many short rows) or a block; rows longer than VECS pieces of 1,024 threads are read twice (LONG).  ALIGNED: pieces lie
 // on 16 bytes; else their entries are read one by one.
-template <typename T> struct Piece { static constexpr int N = 16 / (int)sizeof(T); };
-template <typename T, bool ALIGNED> __device__ __forceinline__ uint4 load_piece(const T* x, int k, int K) {
-  constexpr int N = Piece<T>::N;
-  uint4 v = make_uint4(0u, 0u, 0u, 0u);
-  if (ALIGNED && k + N <= K) return *(const uint4*)(x + k);
-  T* e = (T*)&v;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (k + i < K) e[i] = x[k + i];
-  return v;
-}
-// The largest magnitude so far, of bfloat16 a pair of them (their bits are ordered as float32's are).
-__device__ __forceinline__ uint32_t larger(uint32_t top, const uint4& v, const float*) {
-  constexpr uint32_t M = 0x7fffffffu;
-  return max(max(top, max(v.x & M, v.y & M)), max(v.z & M, v.w & M));
-}
-__device__ __forceinline__ uint32_t larger(uint32_t top, const uint4& v, const bf16*) {
-  constexpr uint32_t M = 0x7fff7fffu;
-  return __vmaxu2(__vmaxu2(top, __vmaxu2(v.x & M, v.y & M)), __vmaxu2(v.z & M, v.w & M));
-}
-__device__ __forceinline__ uint32_t top_bits(uint32_t top, const float*) { return top; }
-__device__ __forceinline__ uint32_t top_bits(uint32_t top, const bf16*) { return max(top << 16, top & 0xffff0000u); }
-
 template <typename T> __device__ __forceinline__ void store_piece(int8_t* q, const uint4& v, const Int8Scale& s, int k, int K) {
   constexpr int N = Piece<T>::N;
   float f[N];
@@ -656,30 +722,41 @@ Plan plan_of(int rows, int N, int K, int sms) {
   return best;
 }
 
-template <bool GLU, typename TO, int BN, int STAGES>
+template <bool GLU, typename TO, typename TX, int BN, int STAGES>
 int launch_few(const CUtensorMap& map, Int8Args p, int blocks, int tiles, cudaStream_t st) {
-  auto kernel = int8_few_kernel<GLU, TO, BN, STAGES>;
+  constexpr bool INSIDE = !std::is_void<TX>::value;
+  auto kernel = int8_few_kernel<GLU, TO, TX, BN, STAGES>;
   p.mine_shift = 2;
   while ((p.splits << p.mine_shift) < BN) ++p.mine_shift;
   const int columns = p.splits > 1 ? p.splits << p.mine_shift : 0;
-  const size_t smem = STAGES * (W_TILE_BYTES + BN * QK) + 1024 + 256 + (size_t)columns * BM * 4;
-  constexpr size_t most = STAGES * (W_TILE_BYTES + BN * QK) + 1024 + 256 + (size_t)(BN < 32 ? 32 : BN) * BM * 4;
+  const size_t smem = STAGES * (W_TILE_BYTES + (INSIDE ? 0 : BN * QK)) + (INSIDE ? p.kb_per_split * BN * QK : 0) + 1024 + 256 + (size_t)columns * BM * 4;
+  constexpr size_t most = INSIDE ? 227 * 1024 - 256 : STAGES * (W_TILE_BYTES + BN * QK) + 1024 + 256 + (size_t)(BN < 32 ? 32 : BN) * BM * 4;
   static_assert(most <= 227 * 1024, "a CTA's shared memory");
+  if (smem > most) return QV_ERR_TOO_LARGE;
   static PerDevice devices;
   const int rc = qv_allow_smem(kernel, most, devices);
   if (rc) return rc;
-  return qv_launch_cluster(kernel, dim3(blocks, tiles, p.splits), dim3(192), smem, st, dim3(1, 1, p.splits), map, p);
+  return qv_launch_cluster(kernel, dim3(blocks, tiles, p.splits), dim3(INSIDE ? 64 + FEW_QUANTIZERS : 192), smem, st, dim3(1, 1, p.splits), map, p);
 }
 
-template <int BN, int DEEP, int SHALLOW>
-int launch_few_as(const CUtensorMap& map, Int8Args p, bool glu, int out_dt, cudaStream_t st) {
-  const int blocks = (p.N + BM - 1) / BM, KT = (p.K + QK - 1) / QK, tiles = (p.rows + BN - 1) / BN, sms = device_sms();
-  p.kb_per_split = (KT + p.splits - 1) / p.splits;
-  while ((p.splits - 1) * p.kb_per_split >= KT) p.splits /= 2, p.kb_per_split = (KT + p.splits - 1) / p.splits;      // none without k blocks
-  // a ring that fills the SM where every CTA finds one for itself (clusters of four find 32 places on 148 SMs), else two CTAs an SM
-  const long long ctas = (long long)blocks * tiles * p.splits;
-  const bool one_wave = p.splits == 4 ? ctas * 8 <= sms * 7 : ctas <= sms;
-#define FEW(GLU, TO) return one_wave ? launch_few<GLU, TO, BN, DEEP>(map, p, blocks, tiles, st) : launch_few<GLU, TO, BN, SHALLOW>(map, p, blocks, tiles, st)
+// k blocks a CTA and whether the CTAs' rings may fill an SM each: where every CTA finds one for itself (clusters of four find 32 places on
+// 148 SMs), else two CTAs share an SM.
+struct Cut { int splits, kb_per_split; bool one_wave; };
+Cut cut_of(const Plan& plan, int rows, int N, int K, int sms) {
+  const int blocks = (N + BM - 1) / BM, KT = (K + QK - 1) / QK, tiles = (rows + plan.bn - 1) / plan.bn;
+  Cut c = {plan.splits, 0, false};
+  c.kb_per_split = (KT + c.splits - 1) / c.splits;
+  while ((c.splits - 1) * c.kb_per_split >= KT) c.splits /= 2, c.kb_per_split = (KT + c.splits - 1) / c.splits;      // none without k blocks
+  const long long ctas = (long long)blocks * tiles * c.splits;
+  c.one_wave = c.splits == 4 ? ctas * 8 <= sms * 7 : ctas <= sms;
+  return c;
+}
+
+template <typename TX, int BN, int DEEP, int SHALLOW>
+int launch_few_as(const CUtensorMap& map, Int8Args p, const Cut& cut, bool glu, int out_dt, cudaStream_t st) {
+  const int blocks = (p.N + BM - 1) / BM, tiles = (p.rows + BN - 1) / BN;
+  p.splits = cut.splits; p.kb_per_split = cut.kb_per_split;
+#define FEW(GLU, TO) return cut.one_wave ? launch_few<GLU, TO, TX, BN, DEEP>(map, p, blocks, tiles, st) : launch_few<GLU, TO, TX, BN, SHALLOW>(map, p, blocks, tiles, st)
   if (glu) {
     if (out_dt == QV_DT_BF16) FEW(true, bf16);
     FEW(true, float);
@@ -687,6 +764,14 @@ int launch_few_as(const CUtensorMap& map, Int8Args p, bool glu, int out_dt, cuda
   if (out_dt == QV_DT_BF16) FEW(false, bf16);
   FEW(false, float);
 #undef FEW
+}
+
+// Whether the kernel for few rows puts them into 8 bits itself: up to 8 rows of which every CTA can read all (32 KB) while its first weights are on
+// their way, with room for its share beside a ring of eight stages, or of five where two CTAs share an SM.  us apart / inside: 1 row, 4096 x
+// 14336 12.9 / 12.1, 4096 x 4096 6.7 / 6.0, 6144 x 4096 7.7 / 7.0; 3 rows, 512 x 512 3.8 / 3.4; 8 rows of 2048 4.7 / 4.6; but 2 rows of 14336 13.1 / 13.5,
+// 8 rows of 4096 7.0 / 7.7, 16 rows of 1024 4.2 / 4.8.
+bool rows_inside(const Plan& plan, const Cut& cut, int rows, int K, int bytes) {
+  return plan.few && plan.bn == 16 && rows <= 8 && (long long)rows * K * bytes <= 32 * 1024 && cut.kb_per_split <= (cut.one_wave ? 32 : 10);
 }
 
 #define INT8_MAX_K 131071             // 128 * 128 * K stays below 2^31
@@ -755,13 +840,15 @@ extern "C" int qv_gemm_int8(void* out, long long ld_out, int out_dt, const int8_
     if (max_tiles <= 0) return 0;
     rt = tile_rows; p.bn = tile_rows; p.row_tiles = max_tiles; p.box = 16;
   } else {
-    const Plan plan = plan_of(rows, N, K, device_sms());
-    p.bn = plan.bn; p.splits = plan.splits;
+    const int sms = device_sms();
+    const Plan plan = plan_of(rows, N, K, sms);
+    p.bn = plan.bn;
     if (plan.few) {
+      const Cut cut = cut_of(plan, rows, N, K, sms);
       if (!make_map_i8(&map, x, rows, K, ld_x, p.bn)) return QV_ERR_UNSUPPORTED;
-      if (p.bn == 16) return launch_few_as<16, 10, 5>(map, p, glu, out_dt, st);
-      if (p.bn == 32) return launch_few_as<32, 9, 4>(map, p, glu, out_dt, st);
-      return launch_few_as<64, 7, 3>(map, p, glu, out_dt, st);
+      if (p.bn == 16) return launch_few_as<void, 16, 10, 5>(map, p, cut, glu, out_dt, st);
+      if (p.bn == 32) return launch_few_as<void, 32, 9, 4>(map, p, cut, glu, out_dt, st);
+      return launch_few_as<void, 64, 7, 3>(map, p, cut, glu, out_dt, st);
     }
     rt = p.bn <= 32 ? 32 : p.bn <= 64 ? 64 : p.bn <= 128 ? 128 : 256;
     p.box = p.bn / 2; p.row_tiles = (rows + p.bn - 1) / p.bn;
@@ -776,10 +863,42 @@ extern "C" int qv_gemm_int8(void* out, long long ld_out, int out_dt, const int8_
   return QV_ERR_UNSUPPORTED;
 }
 
-// The same for rows of float32 or bfloat16 (dense): they are quantized into q (row stride ld_q) and q_scale first.
-extern "C" int qv_linear_int8(void* out, long long ld_out, int out_dt, const void* x, long long ld_x, int x_dt, int8_t* q, long long ld_q, float* q_scale,
-                              const void* w, const float* w_scale, int rows, int N, int K, int act, float limit, float slope, int* err, void* stream) {
-  const int rc = qv_quantize_rows(q, ld_q, q_scale, x, ld_x, x_dt, nullptr, rows, rows, K, stream);
+// Bytes of room that qv_linear_int8 wants for its rows in 8 bits and their scales (0: none).
+extern "C" long long qv_linear_int8_room(int rows, int N, int K, int x_dt) {
+  if (rows <= 0 || N <= 0 || K <= 0) return 0;
+  const int sms = device_sms();
+  const Plan plan = plan_of(rows, N, K, sms);
+  if (plan.few && rows_inside(plan, cut_of(plan, rows, N, K, sms), rows, K, x_dt == QV_DT_F32 ? 4 : 2)) return 0;
+  return (long long)rows * ((K + 15) / 16 * 16 + 4);
+}
+
+// qv_gemm_int8 for rows of float32 or bfloat16 (dense), which are put into 8 bits first: by the product's kernel itself, or in `room`
+// (qv_linear_int8_room bytes on 16), a launch of its own.
+extern "C" int qv_linear_int8(void* out, long long ld_out, int out_dt, const void* x, long long ld_x, int x_dt, void* room, const void* w, const float* w_scale,
+                              int rows, int N, int K, int act, float limit, float slope, int* err, void* stream) {
+  if (rows <= 0 || N <= 0) return 0;
+  const bool glu = act >= 0;
+  if (K <= 0 || ld_x < K || ((uintptr_t)w & 15) || act > 2 || (glu && (N & 31))) return QV_ERR_UNSUPPORTED;
+  if ((out_dt != QV_DT_BF16 && out_dt != QV_DT_F32) || (x_dt != QV_DT_BF16 && x_dt != QV_DT_F32)) return QV_ERR_UNSUPPORTED;
+  if (K > INT8_MAX_K) return QV_ERR_TOO_LARGE;
+  const int sms = device_sms(), bytes = x_dt == QV_DT_F32 ? 4 : 2;
+  const Plan plan = plan_of(rows, N, K, sms);
+  const Cut cut = plan.few ? cut_of(plan, rows, N, K, sms) : Cut{};
+  if (plan.few && rows_inside(plan, cut, rows, K, bytes)) {
+    Int8Args p = {};
+    p.out = out; p.w = (const uint8_t*)w; p.w_scale = w_scale; p.err = err; p.ld_out = ld_out;
+    p.rows = rows; p.N = N; p.K = K; p.experts = 1; p.bn = plan.bn;
+    p.glu = {glu ? act : 0, limit, slope};
+    p.x = x; p.ld_x = ld_x; p.aligned = ((uintptr_t)x & 15) == 0 && (ld_x * bytes) % 16 == 0;
+    CUtensorMap none;
+    memset(&none, 0, sizeof(none));
+    if (x_dt == QV_DT_F32) return launch_few_as<float, 16, 8, 5>(none, p, cut, glu, out_dt, (cudaStream_t)stream);
+    return launch_few_as<bf16, 16, 8, 5>(none, p, cut, glu, out_dt, (cudaStream_t)stream);
+  }
+  if (!room || ((uintptr_t)room & 15)) return QV_ERR_UNSUPPORTED;
+  const long long ld_q = (K + 15) / 16 * 16;
+  float* scale = (float*)((int8_t*)room + rows * ld_q);
+  const int rc = qv_quantize_rows((int8_t*)room, ld_q, scale, x, ld_x, x_dt, nullptr, rows, rows, K, stream);
   if (rc) return rc;
-  return qv_gemm_int8(out, ld_out, out_dt, q, ld_q, q_scale, w, w_scale, rows, N, K, 1, nullptr, 0, 0, act, limit, slope, err, stream);
+  return qv_gemm_int8(out, ld_out, out_dt, (const int8_t*)room, ld_q, scale, w, w_scale, rows, N, K, 1, nullptr, 0, 0, act, limit, slope, err, stream);
 }

@@ -132,13 +132,14 @@ _ARGTYPES = {
     "qv_int8_packed_bytes": [_I, _I, _I],
     "qv_pack_int8": [_V, _V, _L, _I, _I, _I, _V],
     "qv_gemm_int8": [_V, _L, _I, _V, _L, _V, _V, _V, _I, _I, _I, _I, _V, _I, _I, _I, _F, _F, _V, _V],
-    "qv_linear_int8": [_V, _L, _I, _V, _L, _I, _V, _L, _V, _V, _V, _I, _I, _I, _I, _F, _F, _V, _V],
+    "qv_linear_int8_room": [_I, _I, _I, _I],
+    "qv_linear_int8": [_V, _L, _I, _V, _L, _I, _V, _V, _V, _I, _I, _I, _I, _F, _F, _V, _V],
     "qv_norm_gate_add": [_V, _V, _V, _L, _I, _V, _F, _V, _L, _I, _V, _V, _V, _F, _V, _L, _I, _V, _I, _I, _V, _V],
     "qv_argmax": [_V, _V, _I, _I, _L, _V],
     "qv_argmax_ctas": [_I, _I],
     "qv_sample": [_V, _V, _I, _I, _L, _V, _V, _V, _V, _V, _V, _I, _V, _V, _V, _V],
 }
-_RESTYPES = {"qv_error_string": ctypes.c_char_p, "qv_int8_packed_bytes": c_longlong, "qv_packed_weight_bytes": c_longlong, "qv_gemm_bf16_split_slot_bytes": c_longlong,
+_RESTYPES = {"qv_error_string": ctypes.c_char_p, "qv_int8_packed_bytes": c_longlong, "qv_linear_int8_room": c_longlong, "qv_packed_weight_bytes": c_longlong, "qv_gemm_bf16_split_slot_bytes": c_longlong,
              "qv_linear_scan_state_floats": c_longlong, "qv_linear_scan_workspace_bytes": c_longlong, "qv_latent_tc_workspace_bytes": c_longlong, "qv_diff_partial_floats": c_longlong,
              "qv_channel_scan_state_floats": c_longlong, "qv_channel_delta_workspace_floats": c_longlong, "qv_head_delta_state_floats": c_longlong}
 _typed_libs = {}
@@ -1920,13 +1921,19 @@ def _int8_product(out, x, weight: Int8Weight, act: int, limit: float, slope: flo
                               T, weight.n, K, 1, None, 0, 0, act, limit, slope, _err_word(dev), _stream())
         _check(rc, what)
         return
-    ldq = -(-K // 16) * 16
-    room = x.new_empty(T * (ldq + 4), dtype=torch.int8)                        # the rows in 8 bits, then their scales
-    q = room.data_ptr()
-    rc = lib.qv_linear_int8(out.data_ptr(), ld_out, dt, x.data_ptr(), ld, dt_code(x.dtype), q, ldq, q + T * ldq, weight.packed.data_ptr(),
-                            weight.scale.data_ptr(), T, weight.n, K, act, limit, slope, _err_word(dev), _stream())
+    x_dt = dt_code(x.dtype)
+    need = _linear_int8_room(dev, T, weight.n, K, x_dt)
+    room = x.new_empty(need, dtype=torch.int8) if need else None               # the rows in 8 bits, then their scales
+    rc = lib.qv_linear_int8(out.data_ptr(), ld_out, dt, x.data_ptr(), ld, x_dt, _ptr(room), weight.packed.data_ptr(), weight.scale.data_ptr(),
+                            T, weight.n, K, act, limit, slope, _err_word(dev), _stream())
     _check(rc, what)
-    add_launches(1)
+    if need:
+        add_launches(1)
+
+
+@functools.lru_cache(maxsize=1024)          # of the sizes alone (and the device, whose SMs count)
+def _linear_int8_room(dev: int, tokens: int, n: int, k: int, x_dt: int) -> int:
+    return int(_lib("gemm_int8").qv_linear_int8_room(tokens, n, k, x_dt))
 
 
 def gemm_int8(out, x, weight: Int8Weight) -> None:

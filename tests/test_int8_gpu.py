@@ -69,6 +69,17 @@ def test_rows_next_to_the_border(dtype):
     assert_rows(quantized(x), x)
 
 
+def test_rows_of_all_bfloat16_quotients():
+    """Every pair of 8-bit numbers at every distance that leaves anything of the smaller: the quotient is rounded exactly for all of them."""
+    m = torch.arange(128, 256, device="cuda", dtype=F32)
+    entries = torch.cat([m * 2.0 ** -e for e in range(10)])                  # below 2^-8 of the largest nothing but zeros is left
+    for shift in (0, -100, 100):
+        x = torch.where(entries[None] <= m[:, None], entries[None], 0.0)
+        x = torch.cat([m[:, None], x, -x], dim=1) * 2.0 ** shift
+        assert (x.to(BF16).float() == x).all()
+        assert_rows(quantized(x.to(BF16)), x.to(BF16))
+
+
 @pytest.mark.parametrize("k", (64, 77))
 def test_rows_that_are_not_ordinary(k):
     x = normal(gen(1), 12, k)
@@ -127,6 +138,24 @@ def test_product_is_whole_sums_times_scales(tokens, k, n, out):
     again = torch.empty_like(got)
     ops.gemm_int8(again, quantized(x), w)
     assert torch.equal(again, want)
+    ops.check_kernel_errors()
+
+
+@pytest.mark.parametrize("dtype,pad", [(BF16, 0), (BF16, 3), (BF16, 8), (F32, 0), (F32, 1)])
+@pytest.mark.parametrize("tokens,k,n", [(1, 14336, 4096), (1, 1, 1), (2, 100, 3000), (7, 4096, 6144), (16, 1001, 777), (40, 640, 1000), (100, 257, 515), (3, 9000, 130)])
+def test_product_of_rows_as_they_come(tokens, k, n, dtype, pad):
+    """Rows of either type out of a wider tensor, some of zeros and some that are not finite, by whichever kernel puts them into 8 bits."""
+    g = gen(tokens + k + n + pad)
+    x = normal(g, tokens, k + pad, dtype=dtype)[:, pad:]
+    if tokens > 2:
+        x[1] = 0
+        x[2, k - 1] = float("inf")
+    q, s, _ = weight(g, n, k)
+    got = torch.empty((tokens, n), device="cuda", dtype=F32)
+    ops.gemm_int8(got, x, ops.pack_int8(q, s))
+    qx, sx = plain.rows(x)
+    want = plain.product32(qx, sx, q, s)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
     ops.check_kernel_errors()
 
 
