@@ -107,10 +107,11 @@ template <typename TO> __device__ __forceinline__ float gated(float g, float u, 
 // walk over items (a tile of rows, a block of 256 channels):
 //   warp 0      weights and rows by TMA through a ring of STAGES; both CTAs' copies report to the first CTA's barrier
 //   warp 1      of the first CTA: tcgen05.mma, accumulators double-buffered in tensor memory
-//   warps 2..9  epilogue of the item before: scales, activation, stores; two warps share the channels of a quarter of tensor memory and
-//               take groups of 32 rows in turn
+//   warps 2..17 epilogue of the item before: scales, activation, stores; four warps share the channels of a quarter of tensor memory and
+//               take groups of 32 rows in turn.  An item's scales are on their way while the one before is worked on.
 // GLU: a gated product.  TO: the output's type.  RT: rows of a tile at most (a multiple of 32).
-#define PAIR_THREADS 320
+#define PAIR_EPILOGUE 16              // its warps
+#define PAIR_THREADS (64 + 32 * PAIR_EPILOGUE)
 __device__ __forceinline__ uint32_t of_first(const void* p) {      // the address of the same variable in the cluster's first CTA
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
@@ -139,9 +140,9 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
   constexpr int STAGE_BYTES = W_TILE_BYTES + RT / 2 * QK;
   constexpr int TMEM_COLS = 2 * RT;
   uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  constexpr int SCALES = RT < 64 ? 32 : RT / 2;
-  float* scales = (float*)(ring + STAGES * STAGE_BYTES);       // [8 warps][SCALES]: the scales of the rows that a warp takes
-  uint64_t* full = (uint64_t*)(scales + 8 * SCALES);
+  constexpr int TURNS = PAIR_EPILOGUE / 4, SCALES = RT < 32 * TURNS ? 32 : RT / TURNS;
+  float* scales = (float*)(ring + STAGES * STAGE_BYTES);       // [warps][SCALES]: the scales of the rows that a warp takes
+  uint64_t* full = (uint64_t*)(scales + PAIR_EPILOGUE * SCALES);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;               // [2]
   uint64_t* acc_empty = acc_full + 2;                // [2]
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
   const int rank = blockIdx.x & 1;                   // within the pair
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 16); }      // 8 epilogue warps of either CTA
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * PAIR_EPILOGUE); }      // the epilogue's warps of either CTA
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -233,40 +234,53 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
       }
     }
   } else {
-    const int q = warp & 3, turn = (warp - 2) >> 2;            // tensor memory lanes 32 q .. + 31; groups of 32 rows: turn, turn + 2, ...
+    const int q = warp & 3, turn = (warp - 2) >> 2;            // tensor memory lanes 32 q .. + 31; groups of 32 rows: turn, turn + TURNS, ...
     float* xs = scales + (warp - 2) * SCALES;
     const uint32_t done[2] = {of_first(&acc_empty[0]), of_first(&acc_empty[1])};
+    float ws = 0.f, rs[SCALES / 32];                           // of the item that comes next: this lane's channel, this lane's rows
+    auto fetch = [&](const Item& n) {
+      const int ch = (2 * n.fb + rank) * BM + q * 32 + lane;
+      ws = n.e >= 0 && ch < p.N ? p.w_scale[(size_t)n.e * p.N + ch] : 0.f;
+#pragma unroll
+      for (int i = 0; i < SCALES / 32; ++i) {
+        const int row = (i * TURNS + turn) * 32 + lane;
+        rs[i] = n.e >= 0 && row < n.rows ? p.x_scale[n.row0 + row] : 0.f;
+      }
+    };
+    Item w = item_at(p, entry, first, NP);
+    fetch(w);
+    entry = entry_of(p, first + pairs, items, NP);
     int local = 0;
-    for (int item = first; item < items; item += pairs, ++local) {
-      const Item w = item_at(p, entry, item, NP);
-      entry = entry_of(p, item + pairs, items, NP);
-      if (w.e < 0) break;
+    for (int item = first; item < items && w.e >= 0; item += pairs, ++local) {
       const int ch0 = (2 * w.fb + rank) * BM + q * 32;         // this warp's channels
-      const float ws = ch0 + lane < p.N ? p.w_scale[(size_t)w.e * p.N + ch0 + lane] : 0.f;
+      const float w_scale = ws;
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < SCALES; i += 32) {
-        const int row = 2 * i + turn * 32 + lane;
-        xs[i + lane] = row < w.rows ? p.x_scale[w.row0 + row] : 0.f;
-      }
+      for (int i = 0; i < SCALES / 32; ++i) xs[i * 32 + lane] = rs[i];
       __syncwarp();
+      const Item now = w;
+      if (item + pairs < items) {
+        w = item_at(p, entry, item + pairs, NP);
+        fetch(w);
+        entry = entry_of(p, item + 2 * pairs, items, NP);
+      }
       const int b = local & 1;
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[b], (local >> 1) & 1, p.err, 63))) break;     // (the MMA warp then gives up too)
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * RT);
       const int feat = GLU ? (ch0 >> 1) + (lane & 15) : ch0 + lane;
       const bool there = GLU ? 2 * feat < p.N : feat < p.N;
-      TO* out = (TO*)p.out + (size_t)w.row0 * p.ld_out + feat;
+      TO* out = (TO*)p.out + (size_t)now.row0 * p.ld_out + feat;
 #pragma unroll 1
-      for (int c0 = turn * 32; c0 < w.rows; c0 += 64) {
+      for (int c0 = turn * 32; c0 < now.rows; c0 += 32 * TURNS) {
         uint32_t r[32];
         tmem_ld32(taddr + c0, r);
         float v[32];                                 // the rows' scales, then the scaled sums: all of them ahead of the first store
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) *(float4*)&v[j] = *(const float4*)(xs + (c0 >> 6) * 32 + j);
+        for (int j = 0; j < 32; j += 4) *(float4*)&v[j] = *(const float4*)(xs + c0 / (32 * TURNS) * 32 + j);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * v[j] * ws;
+        for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * v[j] * w_scale;
         if (GLU) {
           // a lane of the lower half gives its gate value of the odd row for the up value of the even row
           const int up = lane >> 4;
@@ -276,24 +290,34 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
             const float got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + 1], 16);
             v[j] = gated<TO>(up ? got : v[j], up ? v[j + 1] : got, p.glu);
           }
+          const int left = there ? now.rows - c0 - up : 0;       // rows that this lane still has
+          if (left >= 31) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            if (c0 + j + up < w.rows && there) *o = from_f<TO>(v[j]);
-            o += 2 * p.ld_out;
+            for (int j = 0; j < 32; j += 2, o += 2 * p.ld_out) *o = from_f<TO>(v[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2, o += 2 * p.ld_out)
+              if (j < left) *o = from_f<TO>(v[j]);
           }
-        } else if (there) {
+        } else {
           TO* o = out + (size_t)c0 * p.ld_out;
+          const int left = there ? now.rows - c0 : 0;
+          if (left >= 32) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (c0 + j < w.rows) *o = from_f<TO>(v[j]);
-            o += p.ld_out;
+            for (int j = 0; j < 32; ++j, o += p.ld_out) *o = from_f<TO>(v[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j, o += p.ld_out)
+              if (j < left) *o = from_f<TO>(v[j]);
           }
         }
         __syncwarp();
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(done[b]) : "memory");
+      // relaxed: what the first CTA waits for, the reads of tensor memory, is done; a release would wait for this warp's stores as well (4.7 us an
+      // item of 256 channels x 256 rows instead of %ITEM%)
+      if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(done[b]) : "memory");
     }
   }
   tc_fence_before();
@@ -336,10 +360,12 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t top, const bf16*) { return
 // wait for the kernel ahead (a packed matrix lies still: qv_pack_int8 lets no kernel start before its end).  The CTAs hand their int32 sums
 // to one another through distributed shared memory: each adds up a share of the columns of all of them, scales and stores these; whole
 // sums have no order, so splits change no bit.
-// TX void: the rows are in 8 bits already and come with the weights.  Else they are float32 or bfloat16 and every CTA puts them into 8 bits itself,
-// while its first weights are on their way: eight warps look for the largest entry of every row, then round the CTA's share of k into shared
-// memory.  That is a launch less, and all of it behind the weights' latency, as long as the rows are few and short (see rows_inside).
+// TX void: the rows are in 8 bits already and come with the weights.  Else they are float32 or bfloat16 and every CTA puts its share of them, all
+// rows of its k blocks, into 8 bits itself, while its first weights are on their way: eight warps hold the share in registers, the CTAs of the
+// cluster tell one another the largest magnitudes that they found, and the rounded entries go to shared memory as the products read them.
+// That is a launch less, and mostly behind the weights' latency, as long as a share is small (see rows_inside).
 #define FEW_QUANTIZERS 256
+#define FEW_PIECES 4                  // 16-byte pieces of the share that a thread holds: 16 KB in all
 template <bool GLU, typename TO, typename TX, int BN, int STAGES>
 __global__ void __launch_bounds__(std::is_void<TX>::value ? 192 : 64 + FEW_QUANTIZERS) int8_few_kernel(const __grid_constant__ CUtensorMap map_x, const Int8Args p) {
   extern __shared__ uint8_t smem_raw[];
@@ -355,7 +381,9 @@ __global__ void __launch_bounds__(std::is_void<TX>::value ? 192 : 64 + FEW_QUANT
   uint64_t* rows_there = accum + 1;
   uint32_t* tmem_slot = (uint32_t*)(rows_there + 1);
   __shared__ __align__(16) float xs[BN];                       // the rows' scales
-  __shared__ uint32_t tops[BN];                                // INSIDE: the rows' largest magnitudes
+  __shared__ uint32_t tops[BN];                                // INSIDE: the largest magnitudes of this CTA's share of the rows
+  __shared__ uint32_t all_tops[4][BN];                         // and those of the cluster's CTAs
+  __shared__ Int8Scale row_scale[BN];
   int* sums = (int*)(behind + 256);                            // [splits][columns of this CTA / 4][128 channels][4]: what the cluster hands this CTA
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int KT = (p.K + QK - 1) / QK;
@@ -390,6 +418,11 @@ __global__ void __launch_bounds__(std::is_void<TX>::value ? 192 : 64 + FEW_QUANT
         bulk_load_1d(ring + kb * STAGE_BYTES, w + (size_t)kb * W_TILE_BYTES, &full[kb], W_TILE_BYTES);
       }
     __syncwarp();
+    if (INSIDE && p.splits > 1) {                    // (the two meetings of the cluster's magnitudes)
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    }
     if (!INSIDE) {
       pdl_wait();
       if (leader)
@@ -413,6 +446,11 @@ __global__ void __launch_bounds__(std::is_void<TX>::value ? 192 : 64 + FEW_QUANT
   } else if (warp == 1) {
     const bool leader = elect_one();
     const uint32_t idesc = umma_idesc_i8(BM, BN);
+    if (INSIDE && p.splits > 1) {
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    }
     const bool there = !INSIDE || mbar_wait(rows_there, 0, p.err, 66);
     for (int kb = 0; there && kb < num_kb; ++kb) {
       const int s = kb % STAGES;
@@ -466,57 +504,82 @@ __global__ void __launch_bounds__(std::is_void<TX>::value ? 192 : 64 + FEW_QUANT
       constexpr int N = Piece<TX>::N;
       const TX* x = (const TX*)p.x + (size_t)row0 * p.ld_x;
       if (te < BN) tops[te] = 0u;
-      asm volatile("bar.sync 2, %0;" ::"n"(FEW_QUANTIZERS) : "memory");
-      const int per_row = rows < FEW_QUANTIZERS / 32 ? FEW_QUANTIZERS / 32 / rows : 1;         // warps that share a row
-      const int pieces = (p.K + N - 1) / N, share = (pieces + per_row - 1) / per_row;
-      for (int task = te >> 5; task < rows * per_row; task += FEW_QUANTIZERS / 32) {
-        const int r = task / per_row, from = (task - r * per_row) * share, to = from + share < pieces ? from + share : pieces;
-        const TX* xr = x + (size_t)r * p.ld_x;
-        uint32_t top = 0;
-        for (int i = from + lane; i < to; i += 256) {
-          uint4 v[8];
+      const int per_row = num_kb * (QK / N), pieces = rows * per_row;                          // of the share; a multiple of 16 a row
+      const int down = FEW_QUANTIZERS / per_row, on = FEW_QUANTIZERS - down * per_row;         // from a thread's piece to its next: rows, pieces
+      uint4 v[FEW_PIECES];
+      int row[FEW_PIECES], col[FEW_PIECES];
+      row[0] = te / per_row;
+      col[0] = te - row[0] * per_row;
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            v[u] = i + 32 * u >= to ? make_uint4(0u, 0u, 0u, 0u) : p.aligned ? load_piece<TX, true>(xr, (i + 32 * u) * N, p.K) : load_piece<TX, false>(xr, (i + 32 * u) * N, p.K);
-#pragma unroll
-          for (int u = 0; u < 8; ++u) top = larger(top, v[u], xr);
+      for (int u = 0; u < FEW_PIECES; ++u) {
+        if (u > 0) {
+          col[u] = col[u - 1] + on;
+          row[u] = row[u - 1] + down;
+          if (col[u] >= per_row) { col[u] -= per_row; ++row[u]; }
         }
-        top = __reduce_max_sync(0xffffffffu, top_bits(top, xr));
-        if (lane == 0) atomicMax(&tops[r], top);
+        v[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (row[u] < rows) {
+          const TX* xr = x + (size_t)row[u] * p.ld_x;
+          const int k = kb0 * QK + col[u] * N;
+          v[u] = p.aligned ? load_piece<TX, true>(xr, k, p.K) : load_piece<TX, false>(xr, k, p.K);
+        }
       }
       asm volatile("bar.sync 2, %0;" ::"n"(FEW_QUANTIZERS) : "memory");
-      for (int i = te; i < rows * num_kb * 8; i += FEW_QUANTIZERS) {                           // 16 entries each
-        const int r = i / (num_kb * 8), c = i - r * (num_kb * 8), k = (kb0 + (c >> 3)) * QK + (c & 7) * 16;
-        const TX* xr = x + (size_t)r * p.ld_x;
-        const Int8Scale s = int8_scale(__uint_as_float(tops[r]));
-        uint32_t w[4];
 #pragma unroll
-        for (int u = 0; u < 16 / N; ++u) {
-          const uint4 v = p.aligned ? load_piece<TX, true>(xr, k + u * N, p.K) : load_piece<TX, false>(xr, k + u * N, p.K);
-          const TX* e = (const TX*)&v;
+      for (int u = 0; u < FEW_PIECES; ++u) {
+        if (u * FEW_QUANTIZERS >= pieces) break;
+        uint32_t top = top_bits(larger(0u, v[u], x), x);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));         // sixteen lanes are in one row
+        if ((lane & 15) == 0 && row[u] < rows) atomicMax(&tops[row[u]], top);
+      }
+      asm volatile("bar.sync 2, %0;" ::"n"(FEW_QUANTIZERS) : "memory");
+      if (p.splits > 1) {
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+        if (te < BN * p.splits) {
+          uint32_t remote;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(&all_tops[split][te % BN])), "r"(te / BN));
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(tops[te % BN]) : "memory");
+        }
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      }
+      if (te < BN) {
+        uint32_t top = p.splits > 1 ? 0u : tops[te];
+        for (int s = 0; p.splits > 1 && s < p.splits; ++s) top = max(top, all_tops[s][te]);
+        row_scale[te] = int8_scale(__uint_as_float(top));
+        xs[te] = te < rows ? int8_step(__uint_as_float(top)) : 0.f;
+      }
+      asm volatile("bar.sync 2, %0;" ::"n"(FEW_QUANTIZERS) : "memory");
+#pragma unroll
+      for (int u = 0; u < FEW_PIECES; ++u) {
+        if (u * FEW_QUANTIZERS >= pieces) break;
+        if (row[u] < rows) {
+          const TX* e = (const TX*)&v[u];
           float f[N];
 #pragma unroll
           for (int m = 0; m < N; ++m) f[m] = to_f(e[m]);
-          uint32_t part[N / 4];
-          int8_pack<sizeof(TX) == 2, N>(f, s, part);
-#pragma unroll
-          for (int m = 0; m < N / 4; ++m) w[u * (N / 4) + m] = part[m];
+          uint32_t w[N / 4];
+          int8_pack<sizeof(TX) == 2, N>(f, row_scale[row[u]], w);
+          const int k = col[u] * N;                  // of the share
+          uint8_t* at = rows8 + (k / QK) * (BN * QK) + row[u] * QK + ((((k % QK) >> 4) ^ (row[u] & 7)) << 4) + (k & 15);
+          if (N == 8) *(uint2*)at = make_uint2(w[0], w[N / 4 - 1]);
+          else *(uint32_t*)at = w[0];
         }
-        *(uint4*)(rows8 + (c >> 3) * BN * QK + r * QK + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the products read them
       mbar_arrive(rows_there);
     }
     if (stores) {
       if (ch0 + lane < p.N) ws = p.w_scale[ch0 + lane];
-      if (te < BN) xs[te] = te >= rows ? 0.f : INSIDE ? int8_step(__uint_as_float(tops[te])) : p.x_scale[row0 + te];
+      if (!INSIDE && te < BN) xs[te] = te < rows ? p.x_scale[row0 + te] : 0.f;
       asm volatile("bar.sync 1, 128;" ::: "memory");
       ok = __all_sync(0xffffffffu, mbar_wait(accum, 0, p.err, 63));
       tc_fence_after();
     }
   }
   const int shift = p.mine_shift, mine = 1 << shift;           // columns a CTA adds up: 4 or more
-  if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  if (!INSIDE && p.splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   if (stores && ok) {
     const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
     const uint32_t to = smem_u32(sums) + (uint32_t)(((split << (shift - 2)) * BM + q * 32 + lane) * 16);
@@ -670,7 +733,7 @@ bool make_map_tiles(CUtensorMap* map, const void* packed, long long tiles) {
 
 template <bool GLU, typename TO, int RT, int STAGES>
 int launch_pair(const CUtensorMap& map_x, const CUtensorMap& map_w, const Int8Args& p, cudaStream_t st) {
-  constexpr int smem = STAGES * (W_TILE_BYTES + RT / 2 * QK) + 8 * (RT < 64 ? 32 : RT / 2) * 4 + 1024 + 256;
+  constexpr int smem = STAGES * (W_TILE_BYTES + RT / 2 * QK) + PAIR_EPILOGUE * (RT < 8 * PAIR_EPILOGUE ? 32 : 4 * RT / PAIR_EPILOGUE) * 4 + 1024 + 256;
   static_assert(smem <= 227 * 1024, "a CTA's shared memory");
   static PerDevice devices;
   auto kernel = int8_pair_kernel<GLU, TO, RT, STAGES>;
@@ -730,7 +793,7 @@ int launch_few(const CUtensorMap& map, Int8Args p, int blocks, int tiles, cudaSt
   while ((p.splits << p.mine_shift) < BN) ++p.mine_shift;
   const int columns = p.splits > 1 ? p.splits << p.mine_shift : 0;
   const size_t smem = STAGES * (W_TILE_BYTES + (INSIDE ? 0 : BN * QK)) + (INSIDE ? p.kb_per_split * BN * QK : 0) + 1024 + 256 + (size_t)columns * BM * 4;
-  constexpr size_t most = INSIDE ? 227 * 1024 - 256 : STAGES * (W_TILE_BYTES + BN * QK) + 1024 + 256 + (size_t)(BN < 32 ? 32 : BN) * BM * 4;
+  constexpr size_t most = INSIDE ? 226 * 1024 : STAGES * (W_TILE_BYTES + BN * QK) + 1024 + 256 + (size_t)(BN < 32 ? 32 : BN) * BM * 4;
   static_assert(most <= 227 * 1024, "a CTA's shared memory");
   if (smem > most) return QV_ERR_TOO_LARGE;
   static PerDevice devices;
@@ -766,12 +829,12 @@ int launch_few_as(const CUtensorMap& map, Int8Args p, const Cut& cut, bool glu, 
 #undef FEW
 }
 
-// Whether the kernel for few rows puts them into 8 bits itself: up to 8 rows of which every CTA can read all (32 KB) while its first weights are on
-// their way, with room for its share beside a ring of eight stages, or of five where two CTAs share an SM.  us apart / inside: 1 row, 4096 x
-// 14336 12.9 / 12.1, 4096 x 4096 6.7 / 6.0, 6144 x 4096 7.7 / 7.0; 3 rows, 512 x 512 3.8 / 3.4; 8 rows of 2048 4.7 / 4.6; but 2 rows of 14336 13.1 / 13.5,
-// 8 rows of 4096 7.0 / 7.7, 16 rows of 1024 4.2 / 4.8.
-bool rows_inside(const Plan& plan, const Cut& cut, int rows, int K, int bytes) {
-  return plan.few && plan.bn == 16 && rows <= 8 && (long long)rows * K * bytes <= 32 * 1024 && cut.kb_per_split <= (cut.one_wave ? 32 : 10);
+// Whether the kernel for few rows puts them into 8 bits itself: up to 8 rows, of which a CTA's share is 16 KB at most, with room for it beside a ring
+// of eight stages, or of five where two CTAs share an SM.  A call by itself is bound by its launches, of which this saves one (8 rows, 6144 x 4096:
+// 16.0 us apart, 10.5 inside); among captured ones, us apart / inside: 1 row, 4096 x 14336 12.7 / 12.6, 4096 x 4096 6.8 / 6.2; 3 rows, 512 x 512 3.8 /
+// 3.1; 8 rows, 2048 x 2048 4.7 / 5.0, 4096 x 4096 7.1 / 7.5, 6144 x 4096 7.9 / 8.7; but 4 rows, 4096 x 14336 13.1 / 14.7, 16 rows, 4096 x 4096 7.1 / 9.1.
+bool rows_inside(const Plan& plan, const Cut& cut, int rows, int bytes) {
+  return plan.few && plan.bn == 16 && rows <= 8 && rows * cut.kb_per_split * QK * bytes <= 16 * 1024 && cut.kb_per_split <= (cut.one_wave ? 32 : 10);
 }
 
 #define INT8_MAX_K 131071             // 128 * 128 * K stays below 2^31
@@ -838,7 +901,7 @@ extern "C" int qv_gemm_int8(void* out, long long ld_out, int out_dt, const int8_
   int rt;
   if (tiles) {
     if (max_tiles <= 0) return 0;
-    rt = tile_rows; p.bn = tile_rows; p.row_tiles = max_tiles; p.box = 16;
+    rt = tile_rows; p.bn = tile_rows; p.row_tiles = max_tiles; p.box = tile_rows >= 64 ? 32 : 16;
   } else {
     const int sms = device_sms();
     const Plan plan = plan_of(rows, N, K, sms);
@@ -868,7 +931,7 @@ extern "C" long long qv_linear_int8_room(int rows, int N, int K, int x_dt) {
   if (rows <= 0 || N <= 0 || K <= 0) return 0;
   const int sms = device_sms();
   const Plan plan = plan_of(rows, N, K, sms);
-  if (plan.few && rows_inside(plan, cut_of(plan, rows, N, K, sms), rows, K, x_dt == QV_DT_F32 ? 4 : 2)) return 0;
+  if (plan.few && rows_inside(plan, cut_of(plan, rows, N, K, sms), rows, x_dt == QV_DT_F32 ? 4 : 2)) return 0;
   return (long long)rows * ((K + 15) / 16 * 16 + 4);
 }
 
@@ -884,7 +947,7 @@ extern "C" int qv_linear_int8(void* out, long long ld_out, int out_dt, const voi
   const int sms = device_sms(), bytes = x_dt == QV_DT_F32 ? 4 : 2;
   const Plan plan = plan_of(rows, N, K, sms);
   const Cut cut = plan.few ? cut_of(plan, rows, N, K, sms) : Cut{};
-  if (plan.few && rows_inside(plan, cut, rows, K, bytes)) {
+  if (plan.few && rows_inside(plan, cut, rows, bytes)) {
     Int8Args p = {};
     p.out = out; p.w = (const uint8_t*)w; p.w_scale = w_scale; p.err = err; p.ld_out = ld_out;
     p.rows = rows; p.N = N; p.K = K; p.experts = 1; p.bn = plan.bn;
