@@ -315,8 +315,8 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
       }
       tc_fence_before();
       __syncwarp();
-      // relaxed: what the first CTA waits for, the reads of tensor memory, is done; a release would wait for this warp's stores as well (4.7 us an
-      // item of 256 channels x 256 rows instead of %ITEM%)
+      // relaxed: what the first CTA waits for, the reads of tensor memory, is done; a release would wait for this warp's stores as well (an item
+      // of 256 channels x 256 rows and one k block: 4.7 us instead of 3.7)
       if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(done[b]) : "memory");
     }
   }
@@ -633,7 +633,9 @@ __global__ void __launch_bounds__(std::is_void<TX>::value ? 192 : 64 + FEW_QUANT
 // One read and one write of the row are all it cannot do without, so a row stays in registers, as stored, between its maximum and its
 // rounding: VECS pieces of 16 bytes a thread, all asked for at once.  A row has a warp (no barrier between its two halves, so that the SM's
 // other rows go on: many short rows) or a block; rows longer than VECS pieces of 1,024 threads are read twice (LONG).  ALIGNED: pieces lie
-// on 16 bytes; else their entries are read one by one.
+// on 16 bytes; else their entries are read one by one.  BLOCKS: how many the registers are to leave room for on an SM.  What bounds
+// it is the instructions and, for many rows, how many are on their way at once: 12,288 rows of 1,408 take 9.9 us (5.2 TB/s) with six pieces a
+// thread and 11.1 with eight; 2,048 rows of 14,336 18.1 us (4.9 TB/s) with three blocks an SM and 20.8 with two.
 template <typename T> __device__ __forceinline__ void store_piece(int8_t* q, const uint4& v, const Int8Scale& s, int k, int K) {
   constexpr int N = Piece<T>::N;
   float f[N];
@@ -653,10 +655,9 @@ template <typename T> __device__ __forceinline__ void store_piece(int8_t* q, con
 }
 
 #define QUANTIZE_WARPS 4              // rows of a block whose rows have a warp each
-template <typename T, int VECS, bool WARP, bool ALIGNED, bool LONG>
-__global__ void __launch_bounds__(WARP ? 32 * QUANTIZE_WARPS : 1024) quantize_rows_kernel(int8_t* __restrict__ q, long long ld_q, float* __restrict__ scale,
-                                                                                         const T* __restrict__ x, long long ld_x,
-                                                                                         const int* __restrict__ row_idx, int rows_in, int rows, int K) {
+template <typename T, int VECS, bool WARP, int THREADS, int BLOCKS, bool ALIGNED, bool LONG>
+__global__ void __launch_bounds__(THREADS, BLOCKS) quantize_rows_kernel(int8_t* __restrict__ q, long long ld_q, float* __restrict__ scale, const T* __restrict__ x,
+                                                                       long long ld_x, const int* __restrict__ row_idx, int rows_in, int rows, int K) {
   constexpr int N = Piece<T>::N;
   __shared__ uint32_t red[32];
   pdl_wait();
@@ -860,16 +861,18 @@ extern "C" int qv_quantize_rows(int8_t* q, long long ld_q, float* scale, const v
   if (T <= 0) return 0;
   if (K <= 0 || ld_q < K || ((uintptr_t)q & 15) || (ld_q & 15) || ld_x < K || (!row_idx && rows_in < T)) return QV_ERR_UNSUPPORTED;
   cudaStream_t st = (cudaStream_t)stream;
-#define QUANTIZE(VECS, WARP, ALIGNED, LONG, THREADS)                                                                                                     \
-  return qv_launch(quantize_rows_kernel<TX, VECS, WARP, ALIGNED, LONG>, dim3(WARP ? (T + QUANTIZE_WARPS - 1) / QUANTIZE_WARPS : T), dim3(THREADS), 0, st, q, \
-                   ld_q, scale, (const TX*)x, ld_x, row_idx, rows_in, T, K)
-#define QUANTIZE_AS(ALIGNED)                                                                   \
-  do {                                                                                         \
-    if (pieces > 4096) QUANTIZE(1, false, ALIGNED, true, 1024);                                \
-    if (few && pieces <= 1024) QUANTIZE(1, false, ALIGNED, false, (pieces + 31) / 32 * 32);    \
-    if (pieces <= 128) QUANTIZE(4, true, ALIGNED, false, 32 * QUANTIZE_WARPS);                 \
-    if (pieces <= 256) QUANTIZE(8, true, ALIGNED, false, 32 * QUANTIZE_WARPS);                 \
-    QUANTIZE(4, false, ALIGNED, false, (pieces + 127) / 128 * 32);                             \
+#define QUANTIZE(VECS, WARP, MOST, BLOCKS, ALIGNED, LONG, THREADS)                                                                                     \
+  return qv_launch(quantize_rows_kernel<TX, VECS, WARP, MOST, BLOCKS, ALIGNED, LONG>, dim3(WARP ? (T + QUANTIZE_WARPS - 1) / QUANTIZE_WARPS : T),      \
+                   dim3(THREADS), 0, st, q, ld_q, scale, (const TX*)x, ld_x, row_idx, rows_in, T, K)
+#define QUANTIZE_AS(ALIGNED)                                                                                  \
+  do {                                                                                                        \
+    if (pieces > 4096) QUANTIZE(1, false, 1024, 1, ALIGNED, true, 1024);                                      \
+    if (few && pieces <= 1024) QUANTIZE(1, false, 1024, 1, ALIGNED, false, (pieces + 31) / 32 * 32);          \
+    if (pieces <= 128) QUANTIZE(4, true, 32 * QUANTIZE_WARPS, 8, ALIGNED, false, 32 * QUANTIZE_WARPS);       \
+    if (pieces <= 192) QUANTIZE(6, true, 32 * QUANTIZE_WARPS, 9, ALIGNED, false, 32 * QUANTIZE_WARPS);        \
+    if (pieces <= 256) QUANTIZE(8, true, 32 * QUANTIZE_WARPS, 8, ALIGNED, false, 32 * QUANTIZE_WARPS);       \
+    if (pieces <= 2048) QUANTIZE(4, false, 512, 3, ALIGNED, false, (pieces + 127) / 128 * 32);                \
+    QUANTIZE(4, false, 1024, 1, ALIGNED, false, (pieces + 127) / 128 * 32);                                   \
   } while (0)
   QV_DISPATCH_DT(x_dt, TX, {
     const int pieces = (K + Piece<TX>::N - 1) / Piece<TX>::N;
