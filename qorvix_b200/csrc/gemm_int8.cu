@@ -107,11 +107,10 @@ template <typename TO> __device__ __forceinline__ float gated(float g, float u, 
 // walk over items (a tile of rows, a block of 256 channels):
 //   warp 0      weights and rows by TMA through a ring of STAGES; both CTAs' copies report to the first CTA's barrier
 //   warp 1      of the first CTA: tcgen05.mma, accumulators double-buffered in tensor memory
-//   warps 2..17 epilogue of the item before: scales, activation, stores; four warps share the channels of a quarter of tensor memory and
-//               take groups of 32 rows in turn.  An item's scales are on their way while the one before is worked on.
+//   warps 2..17 epilogue of the item before: scales, activation, stores; up to four warps share the channels of a quarter of tensor memory
+//               and take groups of 32 rows in turn.  An item's scales are on their way while the one before is worked on.
 // GLU: a gated product.  TO: the output's type.  RT: rows of a tile at most (a multiple of 32).
-#define PAIR_EPILOGUE 16              // its warps
-#define PAIR_THREADS (64 + 32 * PAIR_EPILOGUE)
+__host__ __device__ constexpr int pair_epilogue(int RT) { return RT >= 128 ? 16 : RT / 8; }        // its warps: one for 32 rows of a quarter's channels, up to 16
 __device__ __forceinline__ uint32_t of_first(const void* p) {      // the address of the same variable in the cluster's first CTA
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
@@ -134,15 +133,15 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {       // arrives on
 }
 
 template <bool GLU, typename TO, int RT, int STAGES>
-__global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+__global__ void __launch_bounds__(64 + 32 * pair_epilogue(RT)) int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                  const Int8Args p) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int STAGE_BYTES = W_TILE_BYTES + RT / 2 * QK;
   constexpr int TMEM_COLS = 2 * RT;
   uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  constexpr int TURNS = PAIR_EPILOGUE / 4, SCALES = RT < 32 * TURNS ? 32 : RT / TURNS;
+  constexpr int EPILOGUE = pair_epilogue(RT), TURNS = EPILOGUE / 4, SCALES = RT < 32 * TURNS ? 32 : RT / TURNS;
   float* scales = (float*)(ring + STAGES * STAGE_BYTES);       // [warps][SCALES]: the scales of the rows that a warp takes
-  uint64_t* full = (uint64_t*)(scales + PAIR_EPILOGUE * SCALES);
+  uint64_t* full = (uint64_t*)(scales + EPILOGUE * SCALES);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;               // [2]
   uint64_t* acc_empty = acc_full + 2;                // [2]
@@ -151,7 +150,7 @@ __global__ void __launch_bounds__(PAIR_THREADS) int8_pair_kernel(const __grid_co
   const int rank = blockIdx.x & 1;                   // within the pair
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * PAIR_EPILOGUE); }      // the epilogue's warps of either CTA
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * EPILOGUE); }      // the epilogue's warps of either CTA
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -734,7 +733,7 @@ bool make_map_tiles(CUtensorMap* map, const void* packed, long long tiles) {
 
 template <bool GLU, typename TO, int RT, int STAGES>
 int launch_pair(const CUtensorMap& map_x, const CUtensorMap& map_w, const Int8Args& p, cudaStream_t st) {
-  constexpr int smem = STAGES * (W_TILE_BYTES + RT / 2 * QK) + PAIR_EPILOGUE * (RT < 8 * PAIR_EPILOGUE ? 32 : 4 * RT / PAIR_EPILOGUE) * 4 + 1024 + 256;
+  constexpr int smem = STAGES * (W_TILE_BYTES + RT / 2 * QK) + (RT < 128 ? 32 * pair_epilogue(RT) : 4 * RT) * 4 + 1024 + 256;
   static_assert(smem <= 227 * 1024, "a CTA's shared memory");
   static PerDevice devices;
   auto kernel = int8_pair_kernel<GLU, TO, RT, STAGES>;
@@ -743,7 +742,7 @@ int launch_pair(const CUtensorMap& map_x, const CUtensorMap& map_w, const Int8Ar
   const long long items = (long long)p.row_tiles * ((p.N + 2 * BM - 1) / (2 * BM));
   if (items > 0x40000000LL) return QV_ERR_TOO_LARGE;
   const int pairs = device_sms() / 2;
-  return qv_launch_cluster(kernel, dim3(2 * (unsigned)(items < pairs ? items : pairs)), dim3(PAIR_THREADS), (size_t)smem, st, dim3(2, 1, 1), map_x, map_w, p);
+  return qv_launch_cluster(kernel, dim3(2 * (unsigned)(items < pairs ? items : pairs)), dim3(64 + 32 * pair_epilogue(RT)), (size_t)smem, st, dim3(2, 1, 1), map_x, map_w, p);
 }
 
 template <int RT, int STAGES>

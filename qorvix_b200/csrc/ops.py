@@ -1774,15 +1774,32 @@ INT8_TILE_ROWS = (32, 64, 128, 256)
 
 class Int8Rows:
     """Rows of 8-bit integers, each with a scale: values int8 [T, K] (row stride a multiple of 16, on 16 bytes), scale float32 [T]; the row
-    stands for values * scale."""
-    __slots__ = ("values", "scale")
+    stands for values * scale.  int8_rows makes room for them; their addresses are looked up and checked once, when they are made."""
+    __slots__ = ("shape", "ld", "ptr", "scale_ptr", "dev", "_room", "_values", "_scale")
 
     def __init__(self, values, scale):
-        self.values, self.scale = values, scale
+        shape, strides = values.shape, values.stride()
+        if (values.dtype != torch.int8 or len(shape) != 2 or scale.dtype != torch.float32 or scale.shape != shape[:1] or not scale.is_contiguous()
+                or scale.device != values.device):
+            raise KernelError("8-bit rows are int8 [T, K] with a contiguous float32 scale [T]")
+        T, K = shape
+        if (K > 1 and strides[1] != 1) or (T > 1 and (strides[0] % 16 or strides[0] < K)) or values.data_ptr() % 16:
+            raise KernelError("8-bit rows must start on 16 bytes (int8_rows makes such room)")
+        self.shape, self.ld, self.dev, self._room = (T, K), strides[0] if T > 1 else -(-K // 16) * 16, values.get_device(), None
+        self.ptr, self.scale_ptr, self._values, self._scale = values.data_ptr(), scale.data_ptr(), values, scale
 
     @property
-    def shape(self):
-        return self.values.shape
+    def values(self):
+        if self._values is None:
+            T, K = self.shape
+            self._values = self._room[: T * self.ld].view(T, self.ld)[:, :K]
+        return self._values
+
+    @property
+    def scale(self):
+        if self._scale is None:
+            self._scale = self._room[self.shape[0] * self.ld:].view(torch.float32)
+        return self._scale
 
     @property
     def device(self):
@@ -1791,24 +1808,29 @@ class Int8Rows:
 
 class Int8Weight:
     """A matrix [N, K] of 8-bit integers with a scale a row, or `experts` of them (0: one), laid out for the products (pack_int8)."""
-    __slots__ = ("packed", "scale", "n", "k", "experts")
+    __slots__ = ("packed", "scale", "n", "k", "experts", "dev", "ptr", "scale_ptr")
 
     def __init__(self, packed, scale, n: int, k: int, experts: int = 0):
         self.packed, self.scale, self.n, self.k, self.experts = packed, scale, n, k, experts
+        self.dev, self.ptr, self.scale_ptr = packed.get_device(), packed.data_ptr(), scale.data_ptr()
 
     @property
     def device(self):
         return self.packed.device
 
 
+_current_device = _get_device if _get_device is not None else torch.cuda.current_device
+
+
 def _on_current(*tensors) -> int:
     """The device that launches go to, on which all must live."""
-    _need_cuda(tensors[0])
-    dev = _get_device() if _get_device is not None else torch.cuda.current_device()
+    dev = None
     for t in tensors:
-        if t is not None and t.get_device() != dev:
+        if t is not None:
             _need_cuda(t)
-            raise KernelError(f"kernel operands must live on the current CUDA device ({dev}), not on {t.device}")
+            dev = _current_device() if dev is None else dev
+            if t.get_device() != dev:
+                raise KernelError(f"kernel operands must live on the current CUDA device ({dev}), not on {t.device}")
     return dev
 
 
@@ -1820,32 +1842,27 @@ def _err_word(dev: int) -> int:
     """The address of the device's error word."""
     p = _err_words.get(dev)
     if p is None:
+        if torch.cuda.is_current_stream_capturing() and dev not in _tc_state:
+            raise KernelError("call prepare_products(device) once before the first 8-bit product or norm inside a stream capture")
         p = _err_words[dev] = _tc_buffers(torch.device("cuda", dev))["err"].data_ptr()
     return p
 
 
 def int8_rows(tokens: int, k: int, device) -> Int8Rows:
-    """Room for `tokens` rows of k 8-bit integers."""
-    values = torch.empty((tokens, -(-k // 16) * 16), device=device, dtype=torch.int8)
-    return Int8Rows(values if k % 16 == 0 else values[:, :k], torch.empty(tokens, device=device, dtype=torch.float32))
-
-
-def _int8_rows_checked(rows: Int8Rows) -> Int8Rows:
-    v, s = rows.values, rows.scale
-    shape, strides = v.shape, v.stride()
-    if v.dtype != torch.int8 or len(shape) != 2 or s.dtype != torch.float32 or s.shape != shape[:1] or not s.is_contiguous() or s.device != v.device:
-        raise KernelError("8-bit rows are int8 [T, K] with a contiguous float32 scale [T]")
-    if strides[1] != 1 or (shape[0] > 1 and (strides[0] % 16 or strides[0] < shape[1])) or v.data_ptr() % 16:
-        raise KernelError("8-bit rows must start on 16 bytes (int8_rows makes such room)")
-    return rows
+    """Room for `tokens` rows of k 8-bit integers and their scales."""
+    r = object.__new__(Int8Rows)
+    r.ld = ld = -(-k // 16) * 16
+    r._room = room = torch.empty(tokens * (ld + 4), device=device, dtype=torch.int8)
+    r.shape, r.dev, r.ptr, r._values, r._scale = (tokens, k), room.get_device(), room.data_ptr(), None, None
+    r.scale_ptr = r.ptr + tokens * ld
+    return r
 
 
 def quantize_rows(rows: Int8Rows, x, row_idx=None) -> None:
     """rows[r] = x[r], or x[row_idx[r]], in 8 bits: values = round(127 x / max|x|) (the exact quotient; ties to the even one), scale =
     max|x| / 127.  x float32 or bfloat16, rows may be strided.  A row of zeros has scale 0; one that holds an infinity or a NaN has scale
     NaN; an index outside x's rows gives a row of zeros."""
-    v = _int8_rows_checked(rows).values
-    T, K = v.shape
+    T, K = rows.shape
     shape, strides = x.shape, x.stride()
     if len(shape) != 2 or shape[1] != K or (K > 1 and strides[1] != 1):
         raise KernelError(f"rows of {K} entries wanted, whole in memory, not {tuple(shape)} with strides {strides}")
@@ -1858,15 +1875,11 @@ def quantize_rows(rows: Int8Rows, x, row_idx=None) -> None:
             raise KernelError(f"{row_idx.numel()} row indices do not fill {T} rows")
     if T == 0:
         return
-    _on_current(v, x, row_idx)
-    rc = _lib("gemm_int8").qv_quantize_rows(v.data_ptr(), _ld16(v), rows.scale.data_ptr(), x.data_ptr(), strides[0] if shape[0] > 1 else K, dt_code(x.dtype),
+    if _on_current(x, row_idx) != rows.dev:
+        _on_current(rows.values)
+    rc = _lib("gemm_int8").qv_quantize_rows(rows.ptr, rows.ld, rows.scale_ptr, x.data_ptr(), strides[0] if shape[0] > 1 else K, dt_code(x.dtype),
                                             _ptr(row_idx), shape[0], T, K, _stream())
     _check(rc, "quantize_rows")
-
-
-def _ld16(v) -> int:
-    """The row stride of 8-bit rows; of a single row the next multiple of 16."""
-    return v.stride(0) if v.shape[0] > 1 else -(-v.shape[1] // 16) * 16
 
 
 def pack_int8(values, scale) -> Int8Weight:
@@ -1894,38 +1907,53 @@ def quantize_weight(w) -> Int8Weight:
     return pack_int8(rows.values.reshape(w.shape), rows.scale.reshape(w.shape[:-1]))
 
 
-def _int8_product(out, x, weight: Int8Weight, act: int, limit: float, slope: float, what: str) -> None:
-    rows8 = isinstance(x, Int8Rows)
-    v = _int8_rows_checked(x).values if rows8 else x
-    n = weight.n if act < 0 else weight.n // 2
-    shape, strides = v.shape, v.stride()
-    T = shape[0]
+def _refuse_product(out, x, weight: Int8Weight, act: int, what: str) -> None:
+    """Says what a product refuses (or that there is nothing to do: returns)."""
     if weight.experts:
         raise KernelError(f"{what} takes one matrix; experts' matrices go to moe_experts_int8")
     if act >= 0 and (weight.n % 32 or act > 2):
         raise KernelError(f"{what}: gate and up rows alternate in groups of 16, and act is GLU_SILU, GLU_GELU_TANH or GLU_CLAMPED")
-    if len(shape) != 2 or shape[1] != weight.k or out.shape != (T, n):
-        raise KernelError(f"{what}: rows {tuple(shape)} and a matrix of {weight.n} x {weight.k} do not give {tuple(out.shape)}")
-    out_strides = out.stride()
-    ld_out = out_strides[0] if T > 1 else n
-    if (n > 1 and out_strides[1] != 1) or ld_out < n or (weight.k > 1 and strides[1] != 1):
-        raise KernelError(f"{what}: rows must be whole in memory and must not overlap, not strides {strides} and {out_strides}")
-    if T == 0:
+    v = x.values if isinstance(x, Int8Rows) else x
+    n = weight.n if act < 0 else weight.n // 2
+    if v.dim() != 2 or v.shape[1] != weight.k or tuple(out.shape) != (v.shape[0], n):
+        raise KernelError(f"{what}: rows {tuple(v.shape)} and a matrix of {weight.n} x {weight.k} do not give {tuple(out.shape)}")
+    if v.shape[0] == 0:
         return
-    dev = _on_current(out, v, weight.packed)
-    lib, K, dt = _lib("gemm_int8"), weight.k, _DT.get(out.dtype)
-    dt = dt_code(out.dtype) if dt is None else dt
-    ld = strides[0] if T > 1 else -(-K // 16) * 16
+    if (v.stride(1) != 1 and weight.k > 1) or (out.stride(1) != 1 and n > 1) or (out.shape[0] > 1 and out.stride(0) < n):
+        raise KernelError(f"{what}: rows must be whole in memory and must not overlap, not strides {v.stride()} and {out.stride()}")
+    _on_current(out, v, weight.packed)
+    raise KernelError(f"{what}: the matrix was laid out on another device")
+
+
+def _int8_product(out, x, weight: Int8Weight, act: int, limit: float, slope: float, what: str) -> None:
+    N, K, dev = weight.n, weight.k, weight.dev
+    n = N if act < 0 else N >> 1
+    rows8 = type(x) is Int8Rows
     if rows8:
-        rc = lib.qv_gemm_int8(out.data_ptr(), ld_out, dt, v.data_ptr(), ld, x.scale.data_ptr(), weight.packed.data_ptr(), weight.scale.data_ptr(),
-                              T, weight.n, K, 1, None, 0, 0, act, limit, slope, _err_word(dev), _stream())
+        T, k = x.shape
+        fine = k == K and x.dev == dev
+    else:
+        shape, strides = x.shape, x.stride()
+        T = shape[0]
+        fine = shape == (T, K) and (strides[1] == 1 or K == 1) and x.get_device() == dev
+    out_strides = out.stride()
+    if not (fine and T and out.shape == (T, n) and (out_strides[1] == 1 or n == 1) and (T == 1 or out_strides[0] >= n) and out.get_device() == dev >= 0
+            and dev == _current_device() and not weight.experts and (act < 0 or (act <= 2 and not N & 31))):
+        return _refuse_product(out, x, weight, act, what)
+    ld_out = out_strides[0] if T > 1 else n
+    lib, dt = _lib("gemm_int8"), _DT.get(out.dtype)
+    dt = dt_code(out.dtype) if dt is None else dt
+    if rows8:
+        rc = lib.qv_gemm_int8(out.data_ptr(), ld_out, dt, x.ptr, x.ld, x.scale_ptr, weight.ptr, weight.scale_ptr, T, N, K, 1, None, 0, 0, act, limit, slope,
+                              _err_word(dev), _stream())
         _check(rc, what)
         return
-    x_dt = dt_code(x.dtype)
-    need = _linear_int8_room(dev, T, weight.n, K, x_dt)
+    x_dt = _DT.get(x.dtype)
+    x_dt = dt_code(x.dtype) if x_dt is None else x_dt
+    need = _linear_int8_room(dev, T, N, K, x_dt)
     room = x.new_empty(need, dtype=torch.int8) if need else None               # the rows in 8 bits, then their scales
-    rc = lib.qv_linear_int8(out.data_ptr(), ld_out, dt, x.data_ptr(), ld, x_dt, _ptr(room), weight.packed.data_ptr(), weight.scale.data_ptr(),
-                            T, weight.n, K, act, limit, slope, _err_word(dev), _stream())
+    rc = lib.qv_linear_int8(out.data_ptr(), ld_out, dt, x.data_ptr(), strides[0] if T > 1 else -(-K // 16) * 16, x_dt, room.data_ptr() if need else None,
+                            weight.ptr, weight.scale_ptr, T, N, K, act, limit, slope, _err_word(dev), _stream())
     _check(rc, what)
     if need:
         add_launches(1)
@@ -1959,22 +1987,23 @@ def moe_experts_int8(up, out, rows: Int8Rows, weight: Int8Weight, tiles, act: in
     gemm_int8_glu), False: out [R, N] the products themselves; float32 or bfloat16.  tiles: moe_group's table, made for tiles of `tile_rows`
     rows (moe_int8_tile_rows).  Rows that no tile lists are left as they were."""
     n = weight.n // 2 if up else weight.n
-    v = _int8_rows_checked(rows).values
-    R, K = v.shape
+    R, K = rows.shape
     _i32(tiles, "tiles")
     if not weight.experts or tile_rows not in INT8_TILE_ROWS or tiles.numel() % 3:
         raise KernelError("moe_experts_int8 takes experts' matrices and a table, of three numbers a tile, of tiles of 32, 64, 128 or 256 rows")
     if up and (weight.n % 32 or act not in (GLU_SILU, GLU_GELU_TANH, GLU_CLAMPED)):
         raise KernelError("moe_experts_int8: gate and up rows alternate in groups of 16, and act is GLU_SILU, GLU_GELU_TANH or GLU_CLAMPED")
     if K != weight.k:
-        raise KernelError(f"moe_experts_int8: rows {tuple(v.shape)} do not go with matrices of {weight.n} x {weight.k}")
+        raise KernelError(f"moe_experts_int8: rows {(R, K)} do not go with matrices of {weight.n} x {weight.k}")
     ld_out, out_dt = _rows_of(out, (R, n), "out")
     if R == 0 or tiles.numel() == 0:
         return
-    dev = _on_current(out, v, weight.packed, tiles)
-    rc = _lib("gemm_int8").qv_gemm_int8(out.data_ptr(), ld_out, out_dt, v.data_ptr(), _ld16(v), rows.scale.data_ptr(), weight.packed.data_ptr(),
-                                        weight.scale.data_ptr(), R, weight.n, K, weight.experts, tiles.data_ptr(), tiles.numel() // 3, tile_rows,
-                                        int(act) if up else -1, limit, slope, _err_word(dev), _stream())
+    dev = _on_current(out, tiles, weight.packed)
+    if rows.dev != dev:
+        _on_current(rows.values)
+    rc = _lib("gemm_int8").qv_gemm_int8(out.data_ptr(), ld_out, out_dt, rows.ptr, rows.ld, rows.scale_ptr, weight.ptr, weight.scale_ptr, R, weight.n, K,
+                                        weight.experts, tiles.data_ptr(), tiles.numel() // 3, tile_rows, int(act) if up else -1, limit, slope,
+                                        _err_word(dev), _stream())
     _check(rc, "moe_experts_int8")
 
 
@@ -1985,45 +2014,63 @@ def norm_gate_add(residual, y=None, post_weight=None, post_eps: float = 0.0, gat
     is); out = the new residual, normed with next_weight if there is one.  residual and into float32 [T, d] contiguous; y and gate [T, d]
     float32 or bfloat16 (rows may be strided); the weights, gate_bias and scale float32 [d]; out None, float32, bfloat16 (rows may be strided)
     or Int8Rows (the bfloat16 rows in 8 bits, see quantize_rows)."""
-    rows8 = isinstance(out, Int8Rows)
-    o = _int8_rows_checked(out).values if rows8 else out
-    into = residual if into is None else into
     shape = residual.shape
     T, d = shape
-    dev = _on_current(residual, y, post_weight, gate, gate_bias, scale, next_weight, o, into)
-    if residual.dtype != torch.float32 or not residual.is_contiguous():
-        raise KernelError("the residual stream is contiguous float32 [T, d]")
-    if into is not residual:
-        if into.dtype != torch.float32 or into.shape != shape or not into.is_contiguous():
-            raise KernelError("the new residual stream is contiguous float32 [T, d]")
-        apart = abs(into.data_ptr() - residual.data_ptr())
-        if 0 < apart < 4 * T * d:
-            raise KernelError("the new residual stream lies partly over the old one")
+    if into is None:
+        into = residual
+    dev = residual.get_device()
+    fine = (dev >= 0 and T and d and residual.dtype is _F32 and residual.is_contiguous() and dev == _current_device()
+            and (into is residual or (into.dtype is _F32 and into.shape == shape and into.is_contiguous() and into.get_device() == dev)))
+    wide = (d,)
+    for t in (post_weight, gate_bias, scale, next_weight):
+        fine = fine and (t is None or (t.shape == wide and t.dtype is _F32 and t.is_contiguous() and t.get_device() == dev))
     ld_y = ld_gate = ld_out = d
     y_dt = gate_dt = out_kind = F32
     if y is not None:
         ld_y, y_dt = _rows_of(y, shape, "y")
+        fine = fine and y.get_device() == dev
         if gate is not None:
             ld_gate, gate_dt = _rows_of(gate, shape, "gate")
+            fine = fine and gate.get_device() == dev
     elif post_weight is not None or gate is not None or scale is not None:
         raise KernelError("a norm, a gate or a scale needs a y")
-    if rows8:
-        if o.shape != shape:
-            raise KernelError(f"out must be {tuple(shape)}, not {tuple(o.shape)}")
-        ld_out, out_kind = _ld16(o), 2
-    elif o is not None:
-        ld_out, out_kind = _rows_of(o, shape, "out")
-    for t in (post_weight, gate_bias, scale, next_weight):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != d or not t.is_contiguous()):
-            raise KernelError(f"norms' weights, a gate's bias and a scale are contiguous float32 [{d}]")
+    out_ptr = out_scale = None
+    if type(out) is Int8Rows:
+        if out.shape != shape:
+            raise KernelError(f"out must be {tuple(shape)}, not {out.shape}")
+        ld_out, out_kind, out_ptr, out_scale = out.ld, 2, out.ptr, out.scale_ptr
+        fine = fine and out.dev == dev
+    elif out is not None:
+        ld_out, out_kind = _rows_of(out, shape, "out")
+        out_ptr = out.data_ptr()
+        fine = fine and out.get_device() == dev
     if (gate is None and gate_bias is not None) or (out is None and next_weight is not None):
         raise KernelError("a gate's bias needs a gate, and the next norm's weight rows to write")
-    if T == 0 or d == 0 or (y is None and out is None and into is residual):
+    stream, new = residual.data_ptr(), into.data_ptr()
+    if not fine or 0 < abs(new - stream) < 4 * T * d:
+        return _refuse_norm_gate(residual, into, (y, gate, out.values if type(out) is Int8Rows else out), (post_weight, gate_bias, scale, next_weight))
+    if y is None and out is None and into is residual:
         return
-    rc = _lib("norm_gate").qv_norm_gate_add(
-        residual.data_ptr(), into.data_ptr(), _ptr(y), ld_y, y_dt, _ptr(post_weight), post_eps, _ptr(gate), ld_gate, gate_dt, _ptr(gate_bias), _ptr(scale),
-        _ptr(next_weight), next_eps, _ptr(o), ld_out, out_kind, out.scale.data_ptr() if rows8 else None, T, d, _err_word(dev), _stream())
+    rc = _lib("norm_gate").qv_norm_gate_add(stream, new, _ptr(y), ld_y, y_dt, _ptr(post_weight), post_eps, _ptr(gate), ld_gate, gate_dt, _ptr(gate_bias), _ptr(scale),
+                                            _ptr(next_weight), next_eps, out_ptr, ld_out, out_kind, out_scale, T, d, _err_word(dev), _stream())
     _check(rc, "norm_gate_add")
+
+
+_F32 = torch.float32
+
+
+def _refuse_norm_gate(residual, into, rows, weights) -> None:
+    """Says what norm_gate_add refuses (or that there is nothing to do: returns)."""
+    T, d = residual.shape
+    for t in (residual, into):
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != residual.shape:
+            raise KernelError(f"the {'residual' if t is residual else 'new residual'} stream is contiguous float32 [T, d]")
+    for t in weights:
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (d,) or not t.is_contiguous()):
+            raise KernelError(f"norms' weights, a gate's bias and a scale are contiguous float32 [{d}]")
+    if T and d and 0 < abs(into.data_ptr() - residual.data_ptr()) < 4 * T * d:
+        raise KernelError("the new residual stream lies partly over the old one")
+    _on_current(residual, into, *rows, *weights)
 
 
 def _rows_of(t, shape, name: str):
@@ -2031,7 +2078,8 @@ def _rows_of(t, shape, name: str):
     strides = t.stride()
     if t.shape != shape or (strides[1] != 1 and shape[1] > 1) or (shape[0] > 1 and strides[0] < shape[1]):
         raise KernelError(f"{name} must be {tuple(shape)} with whole rows that do not overlap, not {tuple(t.shape)} with strides {strides}")
-    return (strides[0] if shape[0] > 1 else shape[1]), dt_code(t.dtype)
+    dt = _DT.get(t.dtype)
+    return (strides[0] if shape[0] > 1 else shape[1]), dt_code(t.dtype) if dt is None else dt
 
 
 # ------------------------------------------------------------------ attention

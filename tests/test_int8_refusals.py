@@ -36,10 +36,12 @@ def test_rows():
     refused("2 row indices do not fill 3", ops.quantize_rows, rows(3, 64), x, row_idx=torch.zeros(2, dtype=torch.int32))
     refused("CUDA device", ops.quantize_rows, rows(4, 64), x)
     r = rows(4, 64)
-    refused("contiguous float32 scale", ops.quantize_rows, ops.Int8Rows(r.values, r.scale.double()), x)
-    refused("contiguous float32 scale", ops.quantize_rows, ops.Int8Rows(r.values, r.scale[:3]), x)
-    refused("16 bytes", ops.quantize_rows, ops.Int8Rows(torch.zeros(4, 100, dtype=I8), r.scale), torch.zeros(4, 100, dtype=BF16))
-    refused("16 bytes", ops.quantize_rows, ops.Int8Rows(torch.zeros(4, 128, dtype=I8)[:, 1:65], r.scale), x)
+    refused("contiguous float32 scale", ops.Int8Rows, r.values, r.scale.double())
+    refused("contiguous float32 scale", ops.Int8Rows, r.values, r.scale[:3])
+    refused("contiguous float32 scale", ops.Int8Rows, r.values.float(), r.scale)
+    refused("16 bytes", ops.Int8Rows, torch.zeros(4, 100, dtype=I8), r.scale)
+    refused("16 bytes", ops.Int8Rows, torch.zeros(4, 144, dtype=I8)[:, 1:65], r.scale)
+    refused("16 bytes", ops.Int8Rows, torch.zeros(1, 64, dtype=I8).expand(4, 64), r.scale)
 
 
 def test_packing():
