@@ -7,7 +7,8 @@
 //
 // The matrix is packed in 16 KB tiles of 128 rows x 128 k, the shared-memory image the product reads (128-byte rows, 16-byte chunk c of
 // row r at chunk c ^ (r % 8)), zero where the matrix ends.  It is the 128-row operand and the token rows are the narrow one, so that a
-// thread of the epilogue holds one channel of many tokens, rows are padded to 16 only, and dense and grouped products are one kernel.
+// thread of the epilogue holds one channel of many tokens, few rows cost little padding (to 16, of pairs of SMs to 32), and dense and grouped
+// products are one kernel.
 //
 // Every wait is bounded; one that gives up records a code and the CTA winds down.
 #include "int8_rows.cuh"
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(64 + 32 * pair_epilogue(RT)) int8_pair_kernel(
       bool ok = true;
       for (int item = first; ok && item < items; item += pairs, ++local) {
         const Item w = item_at(p, entry, item, NP);
-      entry = entry_of(p, item + pairs, items, NP);
+        entry = entry_of(p, item + pairs, items, NP);
         if (w.e < 0) break;
         const uint32_t idesc = umma_idesc_i8(2 * BM, (w.rows + 31) & ~31);
         const int b = local & 1;

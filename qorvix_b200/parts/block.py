@@ -70,7 +70,8 @@ def _folds(norm) -> bool:
 def _mark_int8(norm, *readers) -> None:
     """Notes on a norm that everything that reads its rows takes them in 8 bits."""
     if norm is not None and hasattr(norm, "add_norm_int8"):
-        norm.int8_rows = all(getattr(r, "takes_int8_rows", False) for r in readers if r is not None)
+        readers = [r for r in readers if r is not None]
+        norm.int8_rows = bool(readers) and all(getattr(r, "takes_int8_rows", False) for r in readers)
 
 
 class ParallelBlock(Block):

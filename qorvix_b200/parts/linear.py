@@ -33,9 +33,8 @@ def int8_weights(on: bool = True):
 
 
 def wants_int8(weight: torch.Tensor) -> bool:
-    """Whether a matrix [N, K], or matrices [E, N, K], built now go into 8 bits."""
-    return (_int8.get() and weight.is_cuda and weight.dtype == torch.bfloat16 and weight.shape[-2] * weight.shape[-1] >= INT8_LEAST
-            and weight.shape[-1] <= ops.INT8_MAX_K)
+    """Whether a matrix [N, K], or the matrices [E, N, K] of a product over grouped rows, go into 8 bits now."""
+    return _int8.get() and weight.is_cuda and weight.dtype == torch.bfloat16 and weight.numel() >= INT8_LEAST and weight.shape[-1] <= ops.INT8_MAX_K
 
 
 class Linear:

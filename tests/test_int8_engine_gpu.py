@@ -94,6 +94,14 @@ def test_the_matrices_take_half_the_room(model_dir):
     assert stored - int8 > 0.9 * matrices                                                # a byte an entry less, but for the scales
 
 
+def test_the_command_line_takes_them(model_dir, capsys):
+    from qorvix_b200.cli.main import main
+    assert main(["generate", str(model_dir), "--tokens", "1,2,3", "--max", "3", "--temp", "0", "--weights", "int8"]) == 0
+    assert "3 prompt tokens, 3 generated" in capsys.readouterr().out
+    assert main(["bench", str(model_dir), "--prompt", "4", "--gen", "2", "--runs", "1", "--weights", "int8", "--json"]) == 0
+    assert main(["generate", str(model_dir), "--tokens", "1,2,3", "--weights", "int9"]) == 1
+
+
 # ------------------------------------------------------------------ routed experts
 
 @pytest.mark.parametrize("tokens", (1, 7, 70, 400))
