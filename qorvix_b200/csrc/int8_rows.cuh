@@ -1,10 +1,11 @@
 // Rows in 8-bit integers: q_k = round(127 x_k / top), ties to the even one, and the scale top / 127, with top = max_k |x_k|.
 //   top 0:           scale 0, q 0
 //   top not finite:  scale NaN, q 0 (every product with the row is NaN, as it is in floating arithmetic)
-// The quotient is the exact one: q does not depend on how a kernel forms it.  v = x * (127 / top) in float32 is off by at most 2^-22 of itself.
+// The quotient is the exact one: q does not depend on how a kernel forms it.  v = x * (127 / top) in float32 is off by at most 2^-21.8 of itself
+// (2^-22 for the quotient of two steps' error that a thread works out for itself, half a step for it as a number, half for the product).
 //   bfloat16 entries: 127 x / top = a / b with whole a up to 127 * 255 and b up to 255, times a power of two; where it is not a half-integer it
-//     differs from every one by 2^-17 of itself or more.  So v rounded to 20 bits is a half-integer just where the quotient is one, and lies
-//     on the quotient's side of it elsewhere.  No entry needs a second look (one in 200 lies on a border; looking at those cost half
+//     differs from every one by 2^-17 of itself or more.  So v rounded to 20 bits (half a step is 2^-21 of it or more, 2^-20 at most) is a
+//     half-integer just where the quotient is one, and lies on the quotient's side of it elsewhere.  No entry needs a second look (one in 200 lies on a border; looking at those cost half
 //     the time of a pass).
 //   float32 entries: where v comes out nearer than 1e-4 to a border, the exact products decide.
 // What is rounded has then lost half a step of 1/127 of the row's largest entry, no more.
@@ -22,7 +23,7 @@ __device__ __forceinline__ Int8Scale int8_scale(float top) {
   s.live = top > 0.f && top < __int_as_float(0x7f800000);
   s.pre = top < 0x1p-60f ? 0x1p64f : top > 0x1p60f ? 0x1p-64f : 1.f;
   s.top = top * s.pre;        // exact: entries that fall below the normal range are under 2^-60 of top
-  s.inv = s.live ? __fdiv_rn(127.f, s.top) : 0.f;
+  s.inv = s.live ? __fdividef(127.f, s.top) : 0.f;
   return s;
 }
 // What is kept beside the row: top / 127, of which the row's entries are whole multiples.

@@ -61,10 +61,24 @@ template <typename T, bool ALIGNED> __device__ __forceinline__ void store_four(T
   if (i + 2 < d) p[i + 2] = from_f<T>(v.z);
   if (i + 3 < d) p[i + 3] = from_f<T>(v.w);
 }
-__device__ __forceinline__ float sigmoid_of(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }      // within a few steps of 2^-23
-__device__ __forceinline__ float square_sum(float4 v) { return (v.x * v.x + v.y * v.y) + (v.z * v.z + v.w * v.w); }
-__device__ __forceinline__ float4 mul(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
-__device__ __forceinline__ float4 mul(float4 a, float b) { return make_float4(a.x * b, a.y * b, a.z * b, a.w * b); }
+// Arithmetic on two entries an instruction: over many rows the instructions are what bounds the pass next to memory.
+__device__ __forceinline__ float2 lo2(float4 v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 hi2(float4 v) { return make_float2(v.z, v.w); }
+__device__ __forceinline__ float4 both(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
+__device__ __forceinline__ float4 mul(float4 a, float4 b) { return both(mul_pair(lo2(a), lo2(b)), mul_pair(hi2(a), hi2(b))); }
+__device__ __forceinline__ float4 mul(float4 a, float b) { return mul(a, make_float4(b, b, b, b)); }
+__device__ __forceinline__ float4 fma(float4 a, float4 b, float4 c) { return both(fma_pair(lo2(a), lo2(b), lo2(c)), fma_pair(hi2(a), hi2(b), hi2(c))); }
+__device__ __forceinline__ float4 add(float4 a, float b) { return both(add_pair(lo2(a), make_float2(b, b)), add_pair(hi2(a), make_float2(b, b))); }
+__device__ __forceinline__ void add_squares(float2& s, float4 v) { s = fma_pair(hi2(v), hi2(v), fma_pair(lo2(v), lo2(v), s)); }
+__device__ __forceinline__ float exp2_of(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float one_over(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+#define MINUS_LOG2_E (-1.4426950408889634f)
+// sigmoid(g + b) = 1 / (1 + 2^(-log2(e) g - log2(e) b)), `bias` = -log2(e) b: within a few steps of 2^-23; 0 from 2^-126 down.
+__device__ __forceinline__ float4 sigmoid_of(float4 g, float4 bias) {
+  const float4 v = fma(g, make_float4(MINUS_LOG2_E, MINUS_LOG2_E, MINUS_LOG2_E, MINUS_LOG2_E), bias);
+  const float4 e = add(make_float4(exp2_of(v.x), exp2_of(v.y), exp2_of(v.z), exp2_of(v.w)), 1.f);
+  return make_float4(one_over(e.x), one_over(e.y), one_over(e.z), one_over(e.w));
+}
 
 // Sum over the block, the same in every thread; its order depends on the block's size alone.
 __device__ __forceinline__ float block_total(float v, float* red /* >= 32 */) {
@@ -77,8 +91,8 @@ __device__ __forceinline__ float block_total(float v, float* red /* >= 32 */) {
   return warp_sum(lane < nwarp ? red[lane] : 0.f);
 }
 
-// What the row-wide operands hold beside one group of four: post is the norm's weight times the scale; ones (a bias: zeros) stand for what there
-// is not, which changes no bit.
+// What the row-wide operands hold beside one group of four: post is the norm's weight times the scale, bias the gate's times -log2(e); ones (a
+// bias: zeros) stand for what there is not, which changes no bit.
 struct Beside { float4 post, bias; };
 struct NoGate {};                                            // in the place of the gate's type
 __device__ __forceinline__ float4 four_of(float v) { return make_float4(v, v, v, v); }
@@ -86,7 +100,7 @@ template <typename TG, bool ALIGNED> __device__ __forceinline__ Beside beside(co
   Beside w;
   w.post = a.w_post ? load_four<float, ALIGNED>(a.w_post, i, a.d) : four_of(1.f);
   if (a.scale) w.post = mul(w.post, load_four<float, ALIGNED>(a.scale, i, a.d));
-  if constexpr (!std::is_same<TG, NoGate>::value) w.bias = a.gate_bias ? load_four<float, ALIGNED>(a.gate_bias, i, a.d) : four_of(0.f);
+  if constexpr (!std::is_same<TG, NoGate>::value) w.bias = a.gate_bias ? mul(load_four<float, ALIGNED>(a.gate_bias, i, a.d), MINUS_LOG2_E) : four_of(0.f);
   return w;
 }
 template <typename TG, bool ALIGNED> __device__ __forceinline__ float4 load_gate(const TG* g, int i, int d) {
@@ -95,10 +109,9 @@ template <typename TG, bool ALIGNED> __device__ __forceinline__ float4 load_gate
 }
 // The new stream's entries: x + z (times 1 / rms(y), and the norm's weight times the scale) (times the gate).
 template <typename TG> __device__ __forceinline__ float4 new_stream(float4 x, float4 z, float4 g, float inv_rms, const Beside& w) {
-  z = mul(mul(z, inv_rms), w.post);
-  if constexpr (!std::is_same<TG, NoGate>::value)
-    z = mul(z, make_float4(sigmoid_of(g.x + w.bias.x), sigmoid_of(g.y + w.bias.y), sigmoid_of(g.z + w.bias.z), sigmoid_of(g.w + w.bias.w)));
-  return make_float4(x.x + z.x, x.y + z.y, x.z + z.z, x.w + z.w);
+  z = mul(z, inv_rms);
+  if constexpr (!std::is_same<TG, NoGate>::value) z = mul(z, sigmoid_of(g, w.bias));
+  return fma(z, w.post, x);
 }
 __device__ __forceinline__ float4 rounded(float4 v) {
   return make_float4(to_f(from_f<bf16>(v.x)), to_f(from_f<bf16>(v.y)), to_f(from_f<bf16>(v.z)), to_f(from_f<bf16>(v.w)));
@@ -129,19 +142,20 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
   float4 x[FOURS], z[FOURS], g[FOURS];
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
   float4 next_of_one = zero;
-  float post = 1.f, s2 = 0.f;
+  float post = 1.f;
+  float2 s2 = make_float2(0.f, 0.f);
   const bool stores = yr != nullptr || so != sr;
   if (LONG) {
     if (yr && a.w_post) {
-      float ss = 0.f;
-      for (int i = threadIdx.x * 4; i < d; i += step) ss += square_sum(load_four<TY, ALIGNED>(yr, i, d));
-      post = 1.0f / sqrtf(block_total(ss, red) / (float)d + a.eps_post);
+      float2 ss = make_float2(0.f, 0.f);
+      for (int i = threadIdx.x * 4; i < d; i += step) add_squares(ss, load_four<TY, ALIGNED>(yr, i, d));
+      post = 1.0f / sqrtf(block_total(ss.x + ss.y, red) / (float)d + a.eps_post);
     }
     for (int i = threadIdx.x * 4; i < d; i += step) {
       const float4 v = new_stream<TG>(load_four<float, ALIGNED>(sr, i, d), yr ? load_four<TY, ALIGNED>(yr, i, d) : zero, load_gate<TG, ALIGNED>(gr, i, d), post,
                                       beside<TG, ALIGNED>(a, i));
       if (stores) store_four<float, ALIGNED>(so, i, d, v);
-      s2 += square_sum(v);
+      add_squares(s2, v);
     }
   } else {
 #pragma unroll
@@ -160,10 +174,10 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
     }
     next_of_one = w_next;
     if (yr && a.w_post) {
-      float ss = 0.f;
+      float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < FOURS; ++k) ss += square_sum(z[k]);
-      post = 1.0f / sqrtf(block_total(ss, red) / (float)d + a.eps_post);
+      for (int k = 0; k < FOURS; ++k) add_squares(ss, z[k]);
+      post = 1.0f / sqrtf(block_total(ss.x + ss.y, red) / (float)d + a.eps_post);
     }
 #pragma unroll
     for (int k = 0; k < FOURS; ++k) {
@@ -171,12 +185,12 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
       if (i < d) {
         x[k] = new_stream<TG>(x[k], z[k], g[k], post, FOURS == 1 ? w[0] : beside<TG, ALIGNED>(a, i));
         if (stores) store_four<float, ALIGNED>(so, i, d, x[k]);
-        s2 += square_sum(x[k]);
+        add_squares(s2, x[k]);
       }
     }
   }
   if (!a.out) return;
-  const float next = a.w_next ? 1.0f / sqrtf(block_total(s2, red) / (float)d + a.eps_next) : 1.f;
+  const float next = a.w_next ? 1.0f / sqrtf(block_total(s2.x + s2.y, red) / (float)d + a.eps_next) : 1.f;
   auto row = [&](int i, float4 v) {
     return a.w_next ? mul(mul(v, next), FOURS == 1 && !LONG ? next_of_one : load_four<float, ALIGNED>(a.w_next, i, d)) : v;
   };
@@ -223,13 +237,16 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
   }
 }
 
-// Many rows: what bounds the pass is memory, so an SM should never be without loads on the way.  As many blocks as the SMs hold walk over the
-// rows; the rows ahead of the one that a block works on come into shared memory by bulk copies, a ring of `stages` of them (two or more), and the weights,
-// which all rows share, stay in registers.  A row then costs two sums over the block (a barrier each) and its arithmetic.  Every row of
-// every operand on 16 bytes and a multiple of them, rows of up to FOURS groups of THREADS threads, as many blocks on an SM as make 1,280 threads:
-// one block's sums and stores run beside another's.
-// 2,048 rows of 5,120, bfloat16 y, gate and rows: 26.7 us, 5.5 TB/s; 53 with a block a row, which waits for its loads and its sums in turn, 46 with
-// the next row on its way to registers, 33 with weights that took more registers than two blocks find.  The stages do not matter from two on.
+// Many rows: memory bounds the pass, and the instructions nearly do, so an SM should never be without loads on the way and a thread should have
+// little to do beside its entries.  As many blocks as the SMs hold walk over the rows; the row ahead of the one that a block works on comes
+// into shared memory by bulk copies, a ring of `stages` of them (two; one where a row of three float32 operands fills the block's share), and
+// the weights, which all rows share, stay in registers.  A row then costs two sums over the block (a barrier each) and its arithmetic, two
+// entries an instruction.  Every row of every operand on 16 bytes and a multiple of them, rows of up to FOURS groups of THREADS threads, as many
+// blocks on an SM as make 640 threads (768 with no gate and no 8-bit rows, which need fewer registers): one block's sums and stores run beside
+// another's.
+// us, 2,048 rows of 5,120, bfloat16 y and gate: bfloat16 rows 27.8 (5.3 TB/s), 8-bit rows 27.9; with two groups a thread and scalar arithmetic 27.1
+// and 34.5 (8,192 rows of 4,096 without a gate: 61.7 in 8 bits, 86.3 so); 53 with a block a row, which waits for its loads and its sums in turn.
+// Two stages or six: 39.9 and 43.2 for rows of 8,192.
 __device__ __forceinline__ float block_total_of(float v, float* red /* >= 32; read by all since this row's or the last row's barrier */) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
   v = warp_sum(v);
@@ -237,8 +254,9 @@ __device__ __forceinline__ float block_total_of(float v, float* red /* >= 32; re
   __syncthreads();
   return warp_sum(lane < nwarp ? red[lane] : 0.f);
 }
+template <typename TG, int OUT> constexpr __host__ __device__ int rows_threads() { return std::is_same<TG, NoGate>::value && OUT != 2 ? 768 : 640; }   // on an SM
 template <typename TY, typename TG, int OUT, int FOURS, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1280 / THREADS) norm_gate_rows_kernel(const NormGateArgs a, int T, int stages, float inv_d, int* err) {
+__global__ void __launch_bounds__(THREADS, rows_threads<TG, OUT>() / THREADS) norm_gate_rows_kernel(const NormGateArgs a, int T, int stages, float inv_d, int* err) {
   extern __shared__ __align__(128) uint8_t ring[];           // [stages][stream row | y row | gate row]
   __shared__ float red[4][32];                               // of the first sum, the second in rows of either parity, the maximum
   __shared__ uint64_t full[8];
@@ -274,59 +292,77 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) norm_gate_rows_kernel
     wn[k] = i < n4 && has_next ? ((const float4*)a.w_next)[i] : four_of(1.f);
   }
   const bool stores = has_y || a.into != a.stream;
+  typedef typename std::conditional<OUT == 0, float, typename std::conditional<OUT == 1, bf16, int8_t>::type>::type TO;
+  float* into = a.into + (size_t)blockIdx.x * d + 4 * threadIdx.x;
+  TO* out = (TO*)a.out + (size_t)blockIdx.x * a.ld_out + 4 * threadIdx.x;
+  const size_t into_step = (size_t)gridDim.x * d, out_step = (size_t)gridDim.x * a.ld_out;
   bool ok = true;                                            // false: a wait gave up; the rest of this block's rows say nothing, and the error word does
-  int it = 0;
-  for (int t = blockIdx.x; t < T; t += gridDim.x, ++it) {
-    const int s = it % stages;
-    const uint8_t* row = ring + s * stage_bytes;
-    ok = ok && mbar_wait(&full[s], (it / stages) & 1, err, 71);
-    float post = 1.f, s2 = 0.f;
+  int s = 0, odd = 0;
+  uint32_t parity = 0;
+  for (int t = blockIdx.x; t < T; t += gridDim.x, into += into_step, out += out_step, odd ^= 1) {
+    const uint8_t* row = ring + s * stage_bytes + 16 * threadIdx.x;
+    const TY* y = (const TY*)(ring + s * stage_bytes + x_bytes) + 4 * threadIdx.x;
+    const TG* g = (const TG*)(ring + s * stage_bytes + x_bytes + y_bytes) + 4 * (std::is_same<TG, NoGate>::value ? 0 : threadIdx.x);
+    if (ok && !mbar_wait(&full[s], parity, err, 71)) {
+      ok = false;
+      if (threadIdx.x == 0)                                  // no copy outlives the block: the ones behind this have been asked for as well
+        for (int n = s + 1; n < s + stages && t + (long long)(n - s) * gridDim.x < T; ++n) mbar_wait(&full[n % stages], parity ^ (n >= stages), err, 71);
+    }
+    float post = 1.f;
+    float2 s2 = make_float2(0.f, 0.f);
     if (has_post) {
-      float ss = 0.f;
+      float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < FOURS; ++k)
-        if (threadIdx.x + k * step < n4) ss += square_sum(Four<TY>::load((const TY*)(row + x_bytes) + 4 * (threadIdx.x + k * step)));
-      post = rsqrtf(block_total_of(ss, red[0]) * inv_d + a.eps_post);
+        if (threadIdx.x + k * step < n4) add_squares(ss, Four<TY>::load(y + 4 * k * step));
+      post = rsqrtf(block_total_of(ss.x + ss.y, red[0]) * inv_d + a.eps_post);
     }
     float4 v[FOURS];
 #pragma unroll
     for (int k = 0; k < FOURS; ++k) {
-      const int i = threadIdx.x + k * step;
       v[k] = zero;
-      if (i < n4) {
-        v[k] = ((const float4*)row)[i];
-        if (has_y) v[k] = new_stream<TG>(v[k], Four<TY>::load((const TY*)(row + x_bytes) + 4 * i), load_gate<TG, true>((const TG*)(row + x_bytes + y_bytes), 4 * i, d), post, w[k]);
-        s2 += square_sum(v[k]);
-        if (stores) ((float4*)(a.into + (size_t)t * d))[i] = v[k];
+      if (threadIdx.x + k * step < n4) {
+        v[k] = *(const float4*)(row + 16 * k * step);
+        if (has_y) v[k] = new_stream<TG>(v[k], Four<TY>::load(y + 4 * k * step), load_gate<TG, true>(g, 4 * k * step, d), post, w[k]);
+        add_squares(s2, v[k]);
+        if (stores) *(float4*)(into + 4 * k * step) = v[k];
       }
     }
-    const float total = block_total_of(s2, red[1 + (it & 1)]), next = has_next ? rsqrtf(total * inv_d + a.eps_next) : 1.f;
-    if (threadIdx.x == 0 && t + (long long)stages * gridDim.x < T) fetch(t + stages * gridDim.x, s);      // (behind the barrier: the row has been read)
-    uint32_t top = 0;
+    const float total = block_total_of(s2.x + s2.y, red[1 + odd]), next = has_next ? rsqrtf(total * inv_d + a.eps_next) : 1.f;
+    if (threadIdx.x == 0 && ok && t + (long long)stages * gridDim.x < T) fetch(t + stages * gridDim.x, s);      // (behind the barrier: the row has been read)
+    if (++s == stages) s = 0, parity ^= 1;
+    if (!a.out) continue;
+    uint32_t tops = 0;                                       // of the entries' 16 bits, two at a time
+    uint2 h[FOURS];
 #pragma unroll
     for (int k = 0; k < FOURS; ++k) {
-      const int i = threadIdx.x + k * step;
-      if (a.out && i < n4) {
+      if (threadIdx.x + k * step < n4) {
         v[k] = mul(mul(v[k], next), wn[k]);
-        if (OUT == 0) Four<float>::store((float*)a.out + (size_t)t * a.ld_out + 4 * i, v[k]);
-        if (OUT == 1) Four<bf16>::store((bf16*)a.out + (size_t)t * a.ld_out + 4 * i, v[k]);
-        if (OUT == 2) {
-          v[k] = rounded(v[k]);
-          top = larger(top, v[k]);
+        if constexpr (OUT != 2) Four<TO>::store(out + 4 * k * step, v[k]);
+        if constexpr (OUT == 2) {
+          Four<bf16>::store((bf16*)&h[k], v[k]);
+          tops = __vmaxu2(tops, __vmaxu2(h[k].x & 0x7fff7fffu, h[k].y & 0x7fff7fffu));
         }
       }
     }
-    if (OUT == 2) {
+    if constexpr (OUT == 2) {
       const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
-      top = __reduce_max_sync(0xffffffffu, top);
+      const uint32_t top = __reduce_max_sync(0xffffffffu, max(tops << 16, tops & 0xffff0000u));
       if (lane == 0) red[3][warp] = __uint_as_float(top);
       __syncthreads();
       const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < nwarp ? __float_as_uint(red[3][lane]) : 0u));
       const Int8Scale q = int8_scale(most);
       if (threadIdx.x == 0) a.out_scale[t] = int8_step(most);
 #pragma unroll
-      for (int k = 0; k < FOURS; ++k)
-        if (threadIdx.x + k * step < n4) put_int8((int8_t*)a.out + (size_t)t * a.ld_out, 4 * (threadIdx.x + k * step), d, v[k], q);
+      for (int k = 0; k < FOURS; ++k) {
+        if (threadIdx.x + k * step < n4) {
+          const float4 r = Four<bf16>::load((const bf16*)&h[k]);
+          float f[4] = {r.x, r.y, r.z, r.w};
+          uint32_t word[1];
+          int8_pack<true, 4>(f, q, word);
+          *(uint32_t*)(out + 4 * k * step) = word[0];
+        }
+      }
     }
   }
 }
@@ -339,10 +375,11 @@ int launch_norm_gate_rows(const NormGateArgs& a, int T, int sms, int* err, cudaS
   const int rc = qv_allow_smem(kernel, ROOM, devices);
   if (rc) return rc;
   const int threads = (a.d / 4 + 32 * FOURS - 1) / (32 * FOURS) * 32;
-  const int on_sm = 1280 / THREADS, blocks = sms * on_sm;
+  constexpr int ON_SM = rows_threads<TG, OUT>();
+  const int on_sm = ON_SM / threads > 10 ? 10 : ON_SM / threads, blocks = sms * on_sm;      // a stage is 192 bytes a thread at most: on_sm of them find room
   const size_t stage = (size_t)a.d * (4 + (a.y ? sizeof(TY) : 0) + (std::is_same<TG, NoGate>::value ? 0 : sizeof(TG)));
   int stages = (int)((size_t)ROOM / on_sm / stage);
-  stages = stages > 6 ? 6 : stages;
+  stages = stages > 2 ? 2 : stages;
   return qv_launch(kernel, dim3(T < blocks ? T : blocks), dim3(threads), stages * stage, st, a, T, stages, 1.0f / (float)a.d, err);
 }
 
@@ -353,10 +390,10 @@ int launch_norm_gate(const NormGateArgs& a, int T, int* err, cudaStream_t st) {
   const bool pieces = ((uintptr_t)a.y & 15) == 0 && ((uintptr_t)a.gate & 15) == 0 && (a.d * sizeof(TY)) % 16 == 0 && (!a.gate || ((a.d * sizeof(TG)) % 16 == 0 && (a.ld_gate * sizeof(TG)) % 16 == 0)) &&
                       (a.ld_y * sizeof(TY)) % 16 == 0;
   if (ALIGNED && pieces && T > 2 * sms && a.d <= 8192)
-    return fours <= 256    ? launch_norm_gate_rows<TY, TG, OUT, 2, 128>(a, T, sms, err, st)
-           : fours <= 640  ? launch_norm_gate_rows<TY, TG, OUT, 2, 320>(a, T, sms, err, st)
-           : fours <= 1280 ? launch_norm_gate_rows<TY, TG, OUT, 2, 640>(a, T, sms, err, st)
-                           : launch_norm_gate_rows<TY, TG, OUT, 2, 1024>(a, T, sms, err, st);
+    return fours <= 256    ? launch_norm_gate_rows<TY, TG, OUT, 4, 64>(a, T, sms, err, st)
+           : fours <= 640  ? launch_norm_gate_rows<TY, TG, OUT, 4, 160>(a, T, sms, err, st)
+           : fours <= 1280 ? launch_norm_gate_rows<TY, TG, OUT, 4, 320>(a, T, sms, err, st)
+                           : launch_norm_gate_rows<TY, TG, OUT, 4, 512>(a, T, sms, err, st);
 #define NORM_GATE_LAUNCH(FOURS, LONG, THREADS) return qv_launch(norm_gate_kernel<TY, TG, OUT, FOURS, ALIGNED, LONG>, dim3(T), dim3(THREADS), 0, st, a)
   if (fours > 2048) NORM_GATE_LAUNCH(1, true, 1024);
   if (T <= 2 * sms && fours <= 1024) NORM_GATE_LAUNCH(1, false, (fours + 31) / 32 * 32);

@@ -27,7 +27,7 @@ def assert_close(got, want, steps, size):
 
 
 @pytest.mark.parametrize("parts", ("all", "no post", "no gate", "no scale", "no bias", "sum alone", "no y", "no next"))
-@pytest.mark.parametrize("tokens,d,y,gate,out", [(1, 1, F32, F32, F32), (300, 4096, BF16, BF16, BF16), (301, 72, F32, F32, BF16), (700, 2056, BF16, F32, F32), (330, 8192, F32, F32, F32), (3, 64, BF16, F32, BF16), (8, 4096, BF16, F32, BF16), (5, 1001, F32, BF16, F32),
+@pytest.mark.parametrize("tokens,d,y,gate,out", [(1, 1, F32, F32, F32), (300, 4096, BF16, BF16, BF16), (301, 72, F32, F32, BF16), (700, 2056, BF16, F32, F32), (330, 8192, F32, F32, F32), (310, 5120, F32, F32, F32), (1500, 1024, F32, F32, BF16), (3, 64, BF16, F32, BF16), (8, 4096, BF16, F32, BF16), (5, 1001, F32, BF16, F32),
                                                  (70, 2056, BF16, BF16, BF16), (2, 20000, BF16, F32, F32)])
 def test_pass(tokens, d, y, gate, out, parts):
     a = inputs(tokens, d, tokens + d, y, gate)
@@ -50,7 +50,7 @@ def test_pass(tokens, d, y, gate, out, parts):
     assert torch.equal(a["residual"], into) and torch.equal(rows2, rows)
 
 
-@pytest.mark.parametrize("tokens,d", [(1, 64), (8, 4096), (3, 1001), (40, 5120), (2, 20000), (310, 1024), (1300, 136), (297, 8192)])
+@pytest.mark.parametrize("tokens,d", [(1, 64), (8, 4096), (3, 1001), (40, 5120), (2, 20000), (310, 1024), (1300, 136), (297, 8192), (900, 2560), (610, 5120), (3000, 520)])
 def test_rows_in_8_bits_are_those_of_the_bfloat16_rows(tokens, d):
     a = inputs(tokens, d, 7 * tokens + d)
     a["residual"][0] *= 1e-3
