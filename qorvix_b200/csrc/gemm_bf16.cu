@@ -80,8 +80,8 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(
 __device__ __forceinline__ float glu_mul(float g, float u, int act, float limit, float slope) {
   if (act == 0) return silu_mul(g, u);
   if (act == 2) {
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit);
+    g = at_most(g, limit);
+    u = at_most(at_least(u, -limit), limit);
     return __fdividef(g, 1.0f + __expf(-slope * g)) * (u + 1.0f);
   }
   return 0.5f * g * (1.0f + tanhf(0.7978845608028654f * fmaf(0.044715f * g * g, g, g))) * u;

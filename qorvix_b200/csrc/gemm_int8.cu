@@ -93,8 +93,8 @@ template <typename TO> __device__ __forceinline__ float gated(float g, float u, 
   float arg = g;
   if (a.kind == 1) arg = 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
   if (a.kind == 2) {
-    g = fminf(g, a.limit);
-    u = fminf(fmaxf(u, -a.limit), a.limit) + 1.f;
+    g = at_most(g, a.limit);
+    u = at_most(at_least(u, -a.limit), a.limit) + 1.f;
     arg = a.slope * g;
   }
   if (sizeof(TO) == 2) return __fdividef(g, 1.f + __expf(-arg)) * u;
