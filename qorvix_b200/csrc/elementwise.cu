@@ -527,7 +527,7 @@ extern "C" int qv_add_vector(float* x, const float* v, int T, int d, void* strea
 // relu, 1: the tanh form of GELU.  VEC elements at a time (VEC 4: n and cols multiples of 4, pointers on the vectors' boundaries).
 __device__ __forceinline__ float activation_of(float z, int kind) {
   if (kind == 1) return 0.5f * z * (1.0f + tanhf(0.7978845608028654f * (z + 0.044715f * z * z * z)));
-  const float v = fmaxf(z, 0.f);
+  const float v = at_least(z, 0.f);
   return v * v;
 }
 

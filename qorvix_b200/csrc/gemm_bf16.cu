@@ -90,7 +90,7 @@ __device__ __forceinline__ float glu_mul(float g, float u, int act, float limit,
 // An ungated activation of EPI 2: 0 the square of relu, 1 the tanh form of GELU.
 __device__ __forceinline__ float ungated_act(float z, int act) {
   if (act == 1) return 0.5f * z * (1.0f + tanhf(0.7978845608028654f * fmaf(0.044715f * z * z, z, z)));
-  const float v = fmaxf(z, 0.f);
+  const float v = at_least(z, 0.f);
   return v * v;
 }
 

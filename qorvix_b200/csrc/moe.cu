@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(256) moe_experts_kernel(void* __restrict__ out
       if (UP) {
         ((T*)out_)[(size_t)(row0 + row) * ld_out + n] = from_f<T>(glu_apply(acc1[r][c], acc2[r][c], glu));
       } else if (MODE == 2) {
-        const float g = fmaxf(acc1[r][c], 0.f);
+        const float g = at_least(acc1[r][c], 0.f);
         ((T*)out_)[(size_t)(row0 + row) * ld_out + n] = from_f<T>(g * g);
       } else {
         ((float*)out_)[(size_t)(row0 + row) * ld_out + n] = acc1[r][c];
@@ -888,7 +888,7 @@ __global__ void __launch_bounds__(192) moe_experts_tc_kernel(const __grid_consta
             if (c0 + j >= rows) break;
             const float v = __uint_as_float(r[j]);
             const size_t at = (size_t)(row0 + c0 + j) * p.ld_out + feat;
-            if (MODE == 2) ((bf16*)p.out)[at] = __float2bfloat16_rn(fmaxf(v, 0.f) * fmaxf(v, 0.f));
+            if (MODE == 2) ((bf16*)p.out)[at] = __float2bfloat16_rn(at_least(v, 0.f) * at_least(v, 0.f));
             else ((float*)p.out)[at] = v;
           }
         }

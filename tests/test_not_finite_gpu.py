@@ -1,4 +1,4 @@
-"""Numbers that are not finite through the activations: a NaN stays one through every clamp, so that a token's fault is seen where
+"""Numbers that are not finite through the activations: a NaN stays one through every clamp and every relu, so that a token's fault is seen where
 the token is; infinities do what the formulas say."""
 import pytest
 import torch
@@ -115,7 +115,7 @@ def test_gated_product(tokens, k, f, dtype, act):
     ops.check_kernel_errors()
 
 
-@pytest.mark.parametrize("mode", GLU)
+@pytest.mark.parametrize("mode", GLU + ("relu2",))
 @pytest.mark.parametrize("dtype,tensor_cores", [(F32, False), (BF16, False), (BF16, True)])
 @pytest.mark.parametrize("tokens", (6, 200))
 def test_experts(tokens, dtype, tensor_cores, mode):
@@ -123,7 +123,7 @@ def test_experts(tokens, dtype, tensor_cores, mode):
     E, top, k, f = 4, 2, 128, 64
     x = normal(g, tokens, k, dtype=dtype)
     x[1, 0] = NAN
-    w = [normal(g, E, f, k, dtype=dtype, std=k ** -0.5) for _ in range(2)]
+    w = [normal(g, E, f, k, dtype=dtype, std=k ** -0.5) for _ in range(1 if mode == "relu2" else 2)]
     top_idx = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(t))[:top] for t in range(tokens)]).to(torch.int32).cuda()
     R = tokens * top
     tile_rows = ops.moe_tile_rows(tensor_cores, tokens, R, E)
@@ -131,13 +131,43 @@ def test_experts(tokens, dtype, tensor_cores, mode):
     tiles = torch.empty(3 * ops.moe_max_tiles(R, E, tile_rows), device="cuda", dtype=torch.int32)
     ops.moe_group(row_token, slot_row, tiles, top_idx, scratch, E, tile_rows)
     out = torch.zeros((R, f), device="cuda", dtype=dtype)
-    kw = dict(act=mode, limit=LIMIT, slope=SLOPE)
+    up, kw = (2, {}) if mode == "relu2" else (True, dict(act=mode, limit=LIMIT, slope=SLOPE))
     if tensor_cores:
         p = [ops.moe_pack_experts(m) for m in w]
-        ops.moe_experts_tc(True, out, x, p[0], p[1], row_token, tiles, tile_rows=tile_rows,
+        ops.moe_experts_tc(up, out, x, p[0], p[1] if len(p) > 1 else None, row_token, tiles, tile_rows=tile_rows,
                            room=torch.empty(R * k, device="cuda", dtype=F32), **kw)
     else:
-        ops.moe_experts(True, out, x, w[0], w[1], row_token, tiles, **kw)
+        ops.moe_experts(up, out, x, w[0], w[1] if len(w) > 1 else None, row_token, tiles, **kw)
     bad = row_token == 1
     assert bad.sum() == top and out[bad].isnan().all() and torch.isfinite(out[~bad]).all()
+    ops.check_kernel_errors()
+
+
+# ------------------------------------------------------------------ the square of relu
+
+@pytest.mark.parametrize("dtype", (F32, BF16))
+@pytest.mark.parametrize("cols", (8, 7))
+def test_ungated_activations(dtype, cols):
+    x = normal(gen(cols), 3, cols, dtype=dtype)
+    x[0, 0], x[1, 1], x[1, 2], x[2, 0] = NAN, INF, -INF, -0.0
+    for kind in (ops.ACT_RELU2, ops.ACT_GELU_TANH):
+        out = torch.empty_like(x)
+        ops.activation(out, x, kind)
+        z = x.double()
+        want = torch.relu(z) ** 2 if kind == ops.ACT_RELU2 else 0.5 * z * (1 + torch.tanh(0.7978845608028654 * (z + 0.044715 * z ** 3)))
+        assert torch.equal(out.isnan(), want.isnan()) and out[0, 0].isnan() and out[1, 1] == INF
+
+
+@pytest.mark.parametrize("act", (ops.ACT_RELU2, ops.ACT_GELU_TANH))
+@pytest.mark.parametrize("tokens,k,n,dtype", [(5, 128, 64, BF16), (90, 256, 128, BF16), (300, 512, 256, BF16), (5, 132, 48, BF16), (6, 96, 32, F32)])
+def test_ungated_product(tokens, k, n, dtype, act):
+    g = gen(tokens + k + n)
+    x = normal(g, tokens, k, dtype=dtype)
+    x[1, 0] = NAN
+    w = normal(g, n, k, dtype=dtype, std=k ** -0.5)
+    bad = torch.arange(tokens, device="cuda") == 1
+    for packed in ((None, ops.pack_weight(w)) if dtype == BF16 and k % 8 == 0 else (None,)):
+        got = torch.zeros((tokens, n), device="cuda", dtype=dtype)
+        ops.gemm_act(got, x, w if packed is None else None, packed, n, act)
+        assert got[bad].isnan().all() and torch.isfinite(got[~bad]).all()
     ops.check_kernel_errors()
