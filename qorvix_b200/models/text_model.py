@@ -10,7 +10,7 @@ from typing import List, Optional
 import torch
 
 from ..csrc import ops
-from ..parts.base import Runtime
+from ..parts.base import Runtime, finish_mixer
 from ..parts.linear import Linear, int8_weights
 from ..parts.registry import build_part
 
@@ -28,7 +28,10 @@ class TextModel:
             self.embedding = self.embedder.weight
         # in 8 bits where the runtime says so: the layers' matrices; the embedding and the head stay as stored
         with int8_weights(rt.weights == "int8"):
-            self.blocks = [build_part("block", _BlockView(layer), source, rt) for layer in spec.layers]
+            self.blocks = []
+            for layer in spec.layers:
+                self.blocks.append(build_part("block", _BlockView(layer), source, rt))
+                finish_mixer(getattr(self.blocks[-1], "mixer", None))
         self.final_norm = build_part("norm", spec.final_norm, source, rt)
         self.lm_head = Linear(source.get(spec.lm_head)) if spec.lm_head is not None else Linear(self.embedding)
         self.order: List[int] = list(spec.order)

@@ -3,6 +3,7 @@
 Mixer         forward(x[T,d], ctx, cache) -> [T,d] in the compute dtype; cache_spec() says what
               it keeps per request (cache.spec.PagedKVSpec / FixedStateSpec / None);
               reads_cache_of() names another layer whose cache it reads instead.
+              finish(), if there is one, is called once the block around the mixer has been built.
 FeedForward   forward(x[T,d], ctx) -> [T,d].
               One whose last product has a bias may offer it as output_bias and take with_bias=False: a
               block then adds it in the pass that takes the output.
@@ -103,6 +104,12 @@ class Mixer:
 
     def forward(self, x, ctx, cache):
         raise NotImplementedError
+
+
+def finish_mixer(mixer) -> None:
+    finish = getattr(mixer, "finish", None)
+    if finish is not None:
+        finish()
 
 
 class FeedForward:

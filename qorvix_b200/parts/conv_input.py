@@ -10,7 +10,7 @@ import torch
 from ..cache.manager import CompositeCacheView
 from ..cache.spec import FixedStateSpec
 from ..csrc import ops
-from .base import Mixer
+from .base import Mixer, finish_mixer
 from .registry import build_part, register_part
 
 
@@ -32,6 +32,9 @@ class ConvInput(Mixer):
 
     def reads_cache_of(self):
         return self.inner.reads_cache_of()
+
+    def finish(self):
+        finish_mixer(self.inner)
 
     def forward(self, x, ctx, cache):
         views = cache.views

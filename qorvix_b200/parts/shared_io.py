@@ -8,6 +8,9 @@ the compute type into `out`, which may be a column slice of a wider buffer, time
 output matrices one product over the concatenated activations.  A block may also hand it further rows that read the same
 input (`take_extra_rows`), whose float32 result it leaves in `extra_out` after every forward: the gate of the block's
 residual, for instance.
+
+The products are made once the block around the mixer is complete (`finish`) and all rows have been handed over, or at the first step of a
+mixer that was built by itself; in 8 bits where the runtime says so.
 """
 from __future__ import annotations
 
@@ -15,7 +18,7 @@ import torch
 
 from ..csrc import ops
 from .base import Mixer
-from .linear import Linear
+from .linear import Linear, int8_weights
 
 
 def stack_rows(mats):
@@ -47,13 +50,18 @@ class SharedIOMixer(Mixer):
     def take_extra_rows(self, weight: torch.Tensor) -> None:
         """Further rows [n, hidden] for the input product; their float32 result is `extra_out` after forward()."""
         if self._in is not None:
-            raise RuntimeError("extra rows must be handed over before the first step")
+            raise RuntimeError("extra rows must be handed over before the products are made")
         self._extra = weight
+
+    def finish(self) -> None:
+        if self._in is None:
+            self._build()
 
     def _build(self):
         mats = [self.in_weights()] + ([self._extra] if self._extra is not None else [])
-        self._in = Linear(stack_rows(mats))
-        self._out = Linear(self.out_weight())
+        with int8_weights(self.rt.weights == "int8"):
+            self._in = Linear(stack_rows(mats))
+            self._out = Linear(self.out_weight())
         b = self.out_bias()
         self._bias = b.float().contiguous() if b is not None else None
         self.release_weights()
@@ -62,8 +70,7 @@ class SharedIOMixer(Mixer):
         """Called once the products hold copies of the matrices: drop what in_weights() / out_weight() kept."""
 
     def forward(self, x, ctx, cache):
-        if self._in is None:
-            self._build()
+        self.finish()
         proj = self._in(x, out_dtype=torch.float32)
         self.extra_out = proj[:, self.in_rows:] if self._extra is not None else None
         heads = torch.empty((x.shape[0], self.out_cols), device=x.device, dtype=x.dtype)

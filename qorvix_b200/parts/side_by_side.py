@@ -8,6 +8,7 @@ from __future__ import annotations
 import torch
 
 from ..csrc import ops
+from .base import finish_mixer
 from .registry import build_part, register_part
 from .shared_io import SharedIOMixer, stack_rows
 
@@ -47,6 +48,13 @@ class SideBySide(SharedIOMixer):
             if b is not None:
                 total = b.float() * s if total is None else total + b.float() * s
         return total
+
+    def finish(self):
+        if self.shared:
+            super().finish()
+        else:
+            finish_mixer(self.left)
+            finish_mixer(self.right)
 
     def release_weights(self):
         self.left.release_weights()
