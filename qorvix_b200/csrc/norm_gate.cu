@@ -7,8 +7,9 @@
 //   stream' = stream + z             (y null: stream' = stream)
 //   rows = stream' / rms(stream') * w_next, in float32, bfloat16 or 8 bits with a scale a row (w_next null: stream' itself)
 //
-// rms(v) = sqrt(mean(v^2) + eps).  Sums and everything between are float32.  8-bit rows are those of the bfloat16 rows, so that they do
-// not depend on whether this pass or qv_quantize_rows made them.
+// rms(v) = sqrt(mean(v^2) + eps).  Sums and everything between are float32.  A row's bits depend on the row and its operands alone, not on how
+// many rows there are: which kernel takes them goes by their number, so all kernels form the same sums in the same order (row_total) and
+// the same root.  8-bit rows are those of the bfloat16 rows, so that they do not depend on whether this pass or qv_quantize_rows made them.
 #include "int8_rows.cuh"
 #include "per_device.h"
 #include "tc_common.cuh"
@@ -30,6 +31,7 @@ struct NormGateArgs {
   float* out_scale;          // 8-bit rows
   long long ld_y, ld_gate, ld_out;
   int d;
+  float inv_d;               // 1 / d
   float eps_post, eps_next;
 };
 
@@ -91,6 +93,33 @@ __device__ __forceinline__ float block_total(float v, float* red /* >= 32 */) {
   return warp_sum(lane < nwarp ? red[lane] : 0.f);
 }
 
+// The sum of a row's squares, the same in every thread, for rows of up to 2,048 groups of four: `sums` threads add up the groups g, g + sums,
+// ... in turn, then comes the tree over them.  FOURS 4: a thread holds just these groups.  FOURS 1: a thread a group; the groups meet in shared memory
+// (`room`), where the first `sums` threads find theirs.  us, rows of 4,096 with a post norm and a gate, a thread a group: 1 row 2.9, 64 rows 3.8, as
+// with a tree over the threads' own sums, which is another order; four groups a thread whatever the number of rows: 4.2 and 6.8.
+__host__ __device__ __forceinline__ int sums_of(int fours) { return (fours + 127) / 128 * 32; }
+template <int FOURS> __device__ __forceinline__ float row_total(const float4 (&v)[FOURS], int fours, float4* room, float* red /* >= 32 */) {
+  float2 s = make_float2(0.f, 0.f);
+  if (FOURS > 1) {
+#pragma unroll
+    for (int k = 0; k < FOURS; ++k) add_squares(s, v[k]);
+    return block_total(s.x + s.y, red);
+  }
+  const int sums = sums_of(fours), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  room[threadIdx.x] = v[0];
+  __syncthreads();
+  if (threadIdx.x < sums) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (threadIdx.x + k * sums < fours) add_squares(s, room[threadIdx.x + k * sums]);
+    const float t = warp_sum(s.x + s.y);
+    if (lane == 0) red[warp] = t;
+  }
+  __syncthreads();
+  return warp_sum(lane < sums / 32 ? red[lane] : 0.f);
+}
+__device__ __forceinline__ float one_over_rms(float total, float inv_d, float eps) { return rsqrtf(fmaf(total, inv_d, eps)); }
+
 // What the row-wide operands hold beside one group of four: post is the norm's weight times the scale, bias the gate's times -log2(e); ones (a
 // bias: zeros) stand for what there is not, which changes no bit.
 struct Beside { float4 post, bias; };
@@ -132,9 +161,10 @@ __device__ __forceinline__ void put_int8(int8_t* o, int i, int d, float4 v, cons
 template <typename TY, typename TG, int OUT, int FOURS, bool ALIGNED, bool LONG>
 __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(const NormGateArgs a) {
   __shared__ float red[32];
+  __shared__ float4 room[FOURS == 1 && !LONG ? 1024 : 1];
   pdl_wait();
   pdl_launch_dependents();
-  const int t = blockIdx.x, d = a.d, step = blockDim.x * 4;
+  const int t = blockIdx.x, d = a.d, fours = (d + 3) / 4, step = blockDim.x * 4;
   const float* sr = a.stream + (size_t)t * d;
   float* so = a.into + (size_t)t * d;
   const TY* yr = a.y ? (const TY*)a.y + (size_t)t * a.ld_y : nullptr;
@@ -142,21 +172,22 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
   float4 x[FOURS], z[FOURS], g[FOURS];
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
   float4 next_of_one = zero;
-  float post = 1.f;
-  float2 s2 = make_float2(0.f, 0.f);
+  float post = 1.f, total = 0.f;                     // total: of the new stream's squares
   const bool stores = yr != nullptr || so != sr;
   if (LONG) {
     if (yr && a.w_post) {
       float2 ss = make_float2(0.f, 0.f);
       for (int i = threadIdx.x * 4; i < d; i += step) add_squares(ss, load_four<TY, ALIGNED>(yr, i, d));
-      post = 1.0f / sqrtf(block_total(ss.x + ss.y, red) / (float)d + a.eps_post);
+      post = one_over_rms(block_total(ss.x + ss.y, red), a.inv_d, a.eps_post);
     }
+    float2 s2 = make_float2(0.f, 0.f);
     for (int i = threadIdx.x * 4; i < d; i += step) {
-      const float4 v = new_stream<TG>(load_four<float, ALIGNED>(sr, i, d), yr ? load_four<TY, ALIGNED>(yr, i, d) : zero, load_gate<TG, ALIGNED>(gr, i, d), post,
-                                      beside<TG, ALIGNED>(a, i));
+      float4 v = load_four<float, ALIGNED>(sr, i, d);
+      if (yr) v = new_stream<TG>(v, load_four<TY, ALIGNED>(yr, i, d), load_gate<TG, ALIGNED>(gr, i, d), post, beside<TG, ALIGNED>(a, i));
       if (stores) store_four<float, ALIGNED>(so, i, d, v);
       add_squares(s2, v);
     }
+    total = block_total(s2.x + s2.y, red);
   } else {
 #pragma unroll
     for (int k = 0; k < FOURS; ++k) {
@@ -173,24 +204,19 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
       if (a.w_next) w_next = load_four<float, ALIGNED>(a.w_next, threadIdx.x * 4, d);
     }
     next_of_one = w_next;
-    if (yr && a.w_post) {
-      float2 ss = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < FOURS; ++k) add_squares(ss, z[k]);
-      post = 1.0f / sqrtf(block_total(ss.x + ss.y, red) / (float)d + a.eps_post);
-    }
+    if (yr && a.w_post) post = one_over_rms(row_total(z, fours, room, red), a.inv_d, a.eps_post);
 #pragma unroll
     for (int k = 0; k < FOURS; ++k) {
       const int i = threadIdx.x * 4 + k * step;
       if (i < d) {
-        x[k] = new_stream<TG>(x[k], z[k], g[k], post, FOURS == 1 ? w[0] : beside<TG, ALIGNED>(a, i));
+        if (yr) x[k] = new_stream<TG>(x[k], z[k], g[k], post, FOURS == 1 ? w[0] : beside<TG, ALIGNED>(a, i));
         if (stores) store_four<float, ALIGNED>(so, i, d, x[k]);
-        add_squares(s2, x[k]);
       }
     }
+    if (a.out && a.w_next) total = row_total(x, fours, room, red);
   }
   if (!a.out) return;
-  const float next = a.w_next ? 1.0f / sqrtf(block_total(s2.x + s2.y, red) / (float)d + a.eps_next) : 1.f;
+  const float next = a.w_next ? one_over_rms(total, a.inv_d, a.eps_next) : 1.f;
   auto row = [&](int i, float4 v) {
     return a.w_next ? mul(mul(v, next), FOURS == 1 && !LONG ? next_of_one : load_four<float, ALIGNED>(a.w_next, i, d)) : v;
   };
@@ -257,7 +283,7 @@ __device__ __forceinline__ float block_total_of(float v, float* red /* >= 32; re
 }
 template <typename TG, int OUT> constexpr __host__ __device__ int rows_threads() { return std::is_same<TG, NoGate>::value && OUT != 2 ? 768 : 640; }   // on an SM
 template <typename TY, typename TG, int OUT, int FOURS, int THREADS>
-__global__ void __launch_bounds__(THREADS, rows_threads<TG, OUT>() / THREADS) norm_gate_rows_kernel(const NormGateArgs a, int T, int stages, float inv_d, int* err) {
+__global__ void __launch_bounds__(THREADS, rows_threads<TG, OUT>() / THREADS) norm_gate_rows_kernel(const NormGateArgs a, int T, int stages, int* err) {
   extern __shared__ __align__(128) uint8_t ring[];           // [stages][stream row | y row | gate row]
   __shared__ float red[4][32];                               // of the first sum, the second in rows of either parity, the maximum
   __shared__ uint64_t full[8];
@@ -316,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, rows_threads<TG, OUT>() / THREADS) no
 #pragma unroll
       for (int k = 0; k < FOURS; ++k)
         if (threadIdx.x + k * step < n4) add_squares(ss, Four<TY>::load(y + 4 * k * step));
-      post = rsqrtf(block_total_of(ss.x + ss.y, red[0]) * inv_d + a.eps_post);
+      post = one_over_rms(block_total_of(ss.x + ss.y, red[0]), a.inv_d, a.eps_post);
     }
     float4 v[FOURS];
 #pragma unroll
@@ -329,7 +355,7 @@ __global__ void __launch_bounds__(THREADS, rows_threads<TG, OUT>() / THREADS) no
         if (stores) *(float4*)(into + 4 * k * step) = v[k];
       }
     }
-    const float total = block_total_of(s2.x + s2.y, red[1 + odd]), next = has_next ? rsqrtf(total * inv_d + a.eps_next) : 1.f;
+    const float total = block_total_of(s2.x + s2.y, red[1 + odd]), next = has_next ? one_over_rms(total, a.inv_d, a.eps_next) : 1.f;
     if (threadIdx.x == 0 && ok && t + (long long)stages * gridDim.x < T) fetch(t + stages * gridDim.x, s);      // (behind the barrier: the row has been read)
     if (++s == stages) s = 0, parity ^= 1;
     if (!a.out) continue;
@@ -375,13 +401,14 @@ int launch_norm_gate_rows(const NormGateArgs& a, int T, int sms, int* err, cudaS
   auto kernel = norm_gate_rows_kernel<TY, TG, OUT, FOURS, THREADS>;
   const int rc = qv_allow_smem(kernel, ROOM, devices);
   if (rc) return rc;
-  const int threads = (a.d / 4 + 32 * FOURS - 1) / (32 * FOURS) * 32;
+  static_assert(FOURS == 4, "sums_of");
+  const int threads = sums_of(a.d / 4);
   constexpr int ON_SM = rows_threads<TG, OUT>();
   const int on_sm = ON_SM / threads > 10 ? 10 : ON_SM / threads, blocks = sms * on_sm;      // a stage is 192 bytes a thread at most: on_sm of them find room
   const size_t stage = (size_t)a.d * (4 + (a.y ? sizeof(TY) : 0) + (std::is_same<TG, NoGate>::value ? 0 : sizeof(TG)));
   int stages = (int)((size_t)ROOM / on_sm / stage);
   stages = stages > 2 ? 2 : stages;
-  return qv_launch(kernel, dim3(T < blocks ? T : blocks), dim3(threads), stages * stage, st, a, T, stages, 1.0f / (float)a.d, err);
+  return qv_launch(kernel, dim3(T < blocks ? T : blocks), dim3(threads), stages * stage, st, a, T, stages, err);
 }
 
 template <typename TY, typename TG, int OUT, bool ALIGNED>
@@ -398,7 +425,7 @@ int launch_norm_gate(const NormGateArgs& a, int T, int* err, cudaStream_t st) {
 #define NORM_GATE_LAUNCH(FOURS, LONG, THREADS) return qv_launch(norm_gate_kernel<TY, TG, OUT, FOURS, ALIGNED, LONG>, dim3(T), dim3(THREADS), 0, st, a)
   if (fours > 2048) NORM_GATE_LAUNCH(1, true, 1024);
   if (T <= 2 * sms && fours <= 1024) NORM_GATE_LAUNCH(1, false, (fours + 31) / 32 * 32);
-  NORM_GATE_LAUNCH(4, false, (fours + 127) / 128 * 32);
+  NORM_GATE_LAUNCH(4, false, sums_of(fours));
 #undef NORM_GATE_LAUNCH
 }
 
@@ -413,7 +440,7 @@ extern "C" int qv_norm_gate_add(const float* stream, float* into, const void* y,
   if ((out_kind == 2) != (out_scale != nullptr) || out_kind < 0 || out_kind > 2) return QV_ERR_UNSUPPORTED;
   NormGateArgs a;
   a.stream = stream; a.into = into; a.y = y; a.w_post = w_post; a.gate = gate; a.gate_bias = gate_bias; a.scale = scale; a.w_next = w_next;
-  a.out = out; a.out_scale = out_scale; a.ld_y = ld_y; a.ld_gate = ld_gate; a.ld_out = ld_out; a.d = d; a.eps_post = eps_post; a.eps_next = eps_next;
+  a.out = out; a.out_scale = out_scale; a.ld_y = ld_y; a.ld_gate = ld_gate; a.ld_out = ld_out; a.d = d; a.inv_d = 1.0f / (float)d; a.eps_post = eps_post; a.eps_next = eps_next;
   cudaStream_t st = (cudaStream_t)cuda_stream;
   const size_t ysz = y_dt == QV_DT_F32 ? 4 : 2, gsz = gate_dt == QV_DT_F32 ? 4 : 2;
   const uintptr_t wide = (uintptr_t)stream | (uintptr_t)into | (uintptr_t)w_post | (uintptr_t)gate_bias | (uintptr_t)scale | (uintptr_t)w_next;
