@@ -72,13 +72,21 @@ __device__ __forceinline__ float4 mul(float4 a, float b) { return mul(a, make_fl
 __device__ __forceinline__ float4 fma(float4 a, float4 b, float4 c) { return both(fma_pair(lo2(a), lo2(b), lo2(c)), fma_pair(hi2(a), hi2(b), hi2(c))); }
 __device__ __forceinline__ float4 add(float4 a, float b) { return both(add_pair(lo2(a), make_float2(b, b)), add_pair(hi2(a), make_float2(b, b))); }
 __device__ __forceinline__ void add_squares(float2& s, float4 v) { s = fma_pair(hi2(v), hi2(v), fma_pair(lo2(v), lo2(v), s)); }
+__device__ __forceinline__ float4 add(float4 a, float4 b) { return both(add_pair(lo2(a), lo2(b)), add_pair(hi2(a), hi2(b))); }
 __device__ __forceinline__ float exp2_of(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float one_over(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
-#define MINUS_LOG2_E (-1.4426950408889634f)
-// sigmoid(g + b) = 1 / (1 + 2^(-log2(e) g - log2(e) b)), `bias` = -log2(e) b: within a few steps of 2^-23; 0 from 2^-126 down.
-__device__ __forceinline__ float4 sigmoid_of(float4 g, float4 bias) {
-  const float4 v = fma(g, make_float4(MINUS_LOG2_E, MINUS_LOG2_E, MINUS_LOG2_E, MINUS_LOG2_E), bias);
-  const float4 e = add(make_float4(exp2_of(v.x), exp2_of(v.y), exp2_of(v.z), exp2_of(v.w)), 1.f);
+// sigmoid(x) = 1 / (1 + exp(-x)), x = g + b rounded once, which moves it by |x| / 2 steps of 2^-23 at most; 0 from 2^-126 down.  float32 y: the accurate
+// exponential, within a few steps.  bfloat16 y: 2^(-log2(e) x), whose argument's roundings move it by as many as |x| steps more, under 2^-16 of itself
+// where it is not 0; y itself has lost up to 2^-9.  (us, 8,192 rows of 4,096, bfloat16 y and gate, 8-bit rows: 86, with the accurate exponential 96.)
+template <typename TY> __device__ __forceinline__ float4 sigmoid_of(float4 g, float4 bias) {
+  float4 x = add(g, bias), e;
+  if (std::is_same<TY, float>::value) {
+    e = make_float4(expf(-x.x), expf(-x.y), expf(-x.z), expf(-x.w));
+  } else {
+    x = mul(x, -1.4426950408889634f);
+    e = make_float4(exp2_of(x.x), exp2_of(x.y), exp2_of(x.z), exp2_of(x.w));
+  }
+  e = add(e, 1.f);
   return make_float4(one_over(e.x), one_over(e.y), one_over(e.z), one_over(e.w));
 }
 
@@ -120,7 +128,7 @@ template <int FOURS> __device__ __forceinline__ float row_total(const float4 (&v
 }
 __device__ __forceinline__ float one_over_rms(float total, float inv_d, float eps) { return rsqrtf(fmaf(total, inv_d, eps)); }
 
-// What the row-wide operands hold beside one group of four: post is the norm's weight times the scale, bias the gate's times -log2(e); ones (a
+// What the row-wide operands hold beside one group of four: post is the norm's weight times the scale, bias the gate's; ones (a
 // bias: zeros) stand for what there is not, which changes no bit.
 struct Beside { float4 post, bias; };
 struct NoGate {};                                            // in the place of the gate's type
@@ -129,7 +137,7 @@ template <typename TG, bool ALIGNED> __device__ __forceinline__ Beside beside(co
   Beside w;
   w.post = a.w_post ? load_four<float, ALIGNED>(a.w_post, i, a.d) : four_of(1.f);
   if (a.scale) w.post = mul(w.post, load_four<float, ALIGNED>(a.scale, i, a.d));
-  if constexpr (!std::is_same<TG, NoGate>::value) w.bias = a.gate_bias ? mul(load_four<float, ALIGNED>(a.gate_bias, i, a.d), MINUS_LOG2_E) : four_of(0.f);
+  if constexpr (!std::is_same<TG, NoGate>::value) w.bias = a.gate_bias ? load_four<float, ALIGNED>(a.gate_bias, i, a.d) : four_of(0.f);
   return w;
 }
 template <typename TG, bool ALIGNED> __device__ __forceinline__ float4 load_gate(const TG* g, int i, int d) {
@@ -137,9 +145,9 @@ template <typename TG, bool ALIGNED> __device__ __forceinline__ float4 load_gate
   else return load_four<TG, ALIGNED>(g, i, d);
 }
 // The new stream's entries: x + z (times 1 / rms(y), and the norm's weight times the scale) (times the gate).
-template <typename TG> __device__ __forceinline__ float4 new_stream(float4 x, float4 z, float4 g, float inv_rms, const Beside& w) {
+template <typename TY, typename TG> __device__ __forceinline__ float4 new_stream(float4 x, float4 z, float4 g, float inv_rms, const Beside& w) {
   z = mul(z, inv_rms);
-  if constexpr (!std::is_same<TG, NoGate>::value) z = mul(z, sigmoid_of(g, w.bias));
+  if constexpr (!std::is_same<TG, NoGate>::value) z = mul(z, sigmoid_of<TY>(g, w.bias));
   return fma(z, w.post, x);
 }
 __device__ __forceinline__ float4 rounded(float4 v) {
@@ -183,7 +191,7 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
     float2 s2 = make_float2(0.f, 0.f);
     for (int i = threadIdx.x * 4; i < d; i += step) {
       float4 v = load_four<float, ALIGNED>(sr, i, d);
-      if (yr) v = new_stream<TG>(v, load_four<TY, ALIGNED>(yr, i, d), load_gate<TG, ALIGNED>(gr, i, d), post, beside<TG, ALIGNED>(a, i));
+      if (yr) v = new_stream<TY, TG>(v, load_four<TY, ALIGNED>(yr, i, d), load_gate<TG, ALIGNED>(gr, i, d), post, beside<TG, ALIGNED>(a, i));
       if (stores) store_four<float, ALIGNED>(so, i, d, v);
       add_squares(s2, v);
     }
@@ -209,7 +217,7 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
     for (int k = 0; k < FOURS; ++k) {
       const int i = threadIdx.x * 4 + k * step;
       if (i < d) {
-        if (yr) x[k] = new_stream<TG>(x[k], z[k], g[k], post, FOURS == 1 ? w[0] : beside<TG, ALIGNED>(a, i));
+        if (yr) x[k] = new_stream<TY, TG>(x[k], z[k], g[k], post, FOURS == 1 ? w[0] : beside<TG, ALIGNED>(a, i));
         if (stores) store_four<float, ALIGNED>(so, i, d, x[k]);
       }
     }
@@ -350,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, rows_threads<TG, OUT>() / THREADS) no
       v[k] = zero;
       if (threadIdx.x + k * step < n4) {
         v[k] = *(const float4*)(row + 16 * k * step);
-        if (has_y) v[k] = new_stream<TG>(v[k], Four<TY>::load(y + 4 * k * step), load_gate<TG, true>(g, 4 * k * step, d), post, w[k]);
+        if (has_y) v[k] = new_stream<TY, TG>(v[k], Four<TY>::load(y + 4 * k * step), load_gate<TG, true>(g, 4 * k * step, d), post, w[k]);
         add_squares(s2, v[k]);
         if (stores) *(float4*)(into + 4 * k * step) = v[k];
       }

@@ -1,4 +1,4 @@
-"""The pass between two sublayers: a row is the same to the bit whatever the other rows of the step are."""
+"""The pass between two sublayers: a row is the same to the bit whatever the other rows of the step are; its gate is as accurate as its types."""
 import pytest
 import torch
 
@@ -79,3 +79,41 @@ def test_logits_of_a_float32_model_do_not_depend_on_the_cut():
         unregister_architecture("SandwichGateLM")
     assert torch.equal(both, alone)
     assert torch.equal(torch.cat(cut), both[:250])
+
+
+# ------------------------------------------------------------------ the gate
+
+@pytest.mark.parametrize("tokens", (3, 700))
+@pytest.mark.parametrize("y", (F32, BF16))
+@pytest.mark.parametrize("gate", (F32, BF16))
+def test_gates_and_biases_that_nearly_cancel(tokens, y, gate):
+    """sigmoid(g + b) where both are large: what counts is the sum x, rounded once (half a step of x, which moves the sigmoid by |x| / 2 steps of
+    2^-23 at most); the exponential's argument in base 2 has three roundings more for bfloat16 y (1.5 |x| steps of 2^-24), the functions, the quotient and
+    the products a few."""
+    d = 512
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    b = (torch.randn(d, generator=g, device="cuda") * 3e3).to(BF16).float()
+    x = torch.randn((tokens, d), generator=g, device="cuda") * 4
+    pre = (x - b).to(gate)
+    a = inputs(tokens, d, 3, y, gate)
+    into = torch.empty_like(a["residual"])
+    ops.norm_gate_add(torch.zeros_like(into), a["y"], gate=pre, gate_bias=b, into=into)
+    arg = pre.double() + b.double()
+    want = a["y"].double() * torch.sigmoid(arg)
+    assert ((into.double() - want).abs() <= want.abs() * (16 + 3 * arg.abs()) * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("tokens", (3, 700))
+def test_a_closed_gate_of_32_bits(tokens):
+    """32-bit y: the accurate functions, within 12 steps of 2^-24 however closed the gate is (the exponential 2 ulp = 4 steps, the sum and the quotient, the
+    products); bfloat16 y: the argument's rounding too, 1.5 |x| steps.  Results below 2^-126 lie 2^-149 apart."""
+    d = 640
+    x = torch.linspace(-85, 20, d, device="cuda").repeat(tokens, 1)
+    a = inputs(tokens, d, 5, F32, F32)
+    for y in (F32, BF16):
+        v = a["y"].to(y)
+        into = torch.empty_like(a["residual"])
+        ops.norm_gate_add(torch.zeros_like(into), v, gate=x, into=into)
+        want = v.double() * torch.sigmoid(x.double())
+        steps = 12 if y == F32 else 16 + 3 * x.double().abs()
+        assert ((into.double() - want).abs() <= want.abs() * steps * 2.0 ** -24 + 2.0 ** -149).all()
