@@ -524,21 +524,21 @@ extern "C" int qv_add_vector(float* x, const float* v, int T, int d, void* strea
 
 // ---------------------------------------------------------------- ungated activations
 // out = act(x + bias) elementwise in place or not, bias one number per column of rows of `cols` (or null); kind 0: the square of
-// relu, 1: the tanh form of GELU.  VEC elements at a time (VEC 4: n and cols multiples of 4, pointers on the vectors' boundaries).
+// relu, 1: the tanh form of GELU.  x in out's type, or float32 sums for bfloat16 out.  VEC elements at a time (VEC 4: n and cols multiples of 4, pointers on the vectors' boundaries).
 __device__ __forceinline__ float activation_of(float z, int kind) {
   if (kind == 1) return 0.5f * z * (1.0f + tanhf(0.7978845608028654f * (z + 0.044715f * z * z * z)));
   const float v = at_least(z, 0.f);
   return v * v;
 }
 
-template <typename T, int VEC>
-__global__ void activation_kernel(T* out, const T* x, const float* __restrict__ bias, size_t n, int cols, int kind) {
+template <typename TX, typename T, int VEC>
+__global__ void activation_kernel(T* out, const TX* x, const float* __restrict__ bias, size_t n, int cols, int kind) {
   pdl_wait();
   pdl_launch_dependents();
   for (size_t i = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * VEC; i < n; i += (size_t)gridDim.x * blockDim.x * VEC) {
     const int c = bias ? (int)(i % (unsigned)cols) : 0;
     if constexpr (VEC == 4) {
-      float4 z = Vec4<T>::load(x + i);
+      float4 z = Vec4<TX>::load(x + i);
       if (bias) {
         const float4 b = *(const float4*)(bias + c);
         z.x += b.x; z.y += b.y; z.z += b.z; z.w += b.w;
@@ -550,16 +550,19 @@ __global__ void activation_kernel(T* out, const T* x, const float* __restrict__ 
   }
 }
 
-extern "C" int qv_activation(void* out, const void* x, const float* bias, long long n, int cols, int kind, int dt, void* stream) {
+extern "C" int qv_activation(void* out, const void* x, const float* bias, long long n, int cols, int kind, int x_dt, int dt, void* stream) {
   if (n <= 0) return 0;
-  if ((kind != 0 && kind != 1) || cols <= 0) return QV_ERR_UNSUPPORTED;
+  if ((kind != 0 && kind != 1) || cols <= 0 || (x_dt != dt && x_dt != QV_DT_F32)) return QV_ERR_UNSUPPORTED;
   const bool vec = n % 4 == 0 && cols % 4 == 0 && (((uintptr_t)out | (uintptr_t)x | (uintptr_t)bias) & 15) == 0;
   const long long work = vec ? n / 4 : n;
   const int blocks = (int)((work + 255) / 256 < 148 * 16 ? (work + 255) / 256 : 148 * 16);
   cudaStream_t st = (cudaStream_t)stream;
-  if (vec)
-    QV_DISPATCH_DT(dt, TT, return qv_launch(activation_kernel<TT, 4>, dim3(blocks), dim3(256), 0, st, (TT*)out, (const TT*)x, bias, (size_t)n, cols, kind));
-  QV_DISPATCH_DT(dt, TT, return qv_launch(activation_kernel<TT, 1>, dim3(blocks), dim3(256), 0, st, (TT*)out, (const TT*)x, bias, (size_t)n, cols, kind));
+#define ACTIVATION(TX, TT)                                                                                                                          \
+  return vec ? qv_launch(activation_kernel<TX, TT, 4>, dim3(blocks), dim3(256), 0, st, (TT*)out, (const TX*)x, bias, (size_t)n, cols, kind)          \
+             : qv_launch(activation_kernel<TX, TT, 1>, dim3(blocks), dim3(256), 0, st, (TT*)out, (const TX*)x, bias, (size_t)n, cols, kind)
+  if (x_dt != dt) QV_DISPATCH_DT(dt, TT, ACTIVATION(float, TT));
+  QV_DISPATCH_DT(dt, TT, ACTIVATION(TT, TT));
+#undef ACTIVATION
   return QV_ERR_UNSUPPORTED;
 }
 

@@ -90,7 +90,7 @@ _ARGTYPES = {
     "qv_scale_sum2": [_V, _V, _V, _V, _V, _I, _I, _I, _I, _V],
     "qv_stream_concat": [_V, _V, _V, _V, _I, _I, _I, _I, _V],
     "qv_add_vector": [_V, _V, _I, _I, _V],
-    "qv_activation": [_V, _V, _V, _L, _I, _I, _I, _V],
+    "qv_activation": [_V, _V, _V, _L, _I, _I, _I, _I, _V],
     "qv_stream_pass": [_V, _V, _V, _V, _I, _V, _V, _V, _V, _F, _V, _I, _I, _I, _I, _I, _I, _V],
     "qv_cache_rows": [_V, _V, _I, _V, _V, _V, _I, _I, _I, _I, _I, _V],
     "qv_diff_prepare_vec": [_I, _I, _I, _I],
@@ -384,11 +384,12 @@ ACT_RELU2, ACT_GELU_TANH = 0, 1
 
 def activation(out, x, kind: int = ACT_RELU2, bias=None) -> None:
     """out = act(x + bias) elementwise (out may be x; bias float32, one per column, or None); kind ACT_RELU2: the square of relu,
-    ACT_GELU_TANH: the tanh form of GELU."""
+    ACT_GELU_TANH: the tanh form of GELU.  x has out's type, or is float32 where out is bfloat16 (another tensor then)."""
     _need_cuda(out, x, bias)
-    assert out.dtype == x.dtype and out.is_contiguous() and x.is_contiguous() and out.numel() == x.numel()
+    assert out.dtype == x.dtype or (x.dtype == torch.float32 and out.dtype == torch.bfloat16)
+    assert out.is_contiguous() and x.is_contiguous() and out.numel() == x.numel()
     assert bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == x.shape[-1])
-    _check(_lib("elementwise").qv_activation(_ptr(out), _ptr(x), _ptr(bias), x.numel(), x.shape[-1], kind, dt_code(x.dtype), _stream()), "activation")
+    _check(_lib("elementwise").qv_activation(_ptr(out), _ptr(x), _ptr(bias), x.numel(), x.shape[-1], kind, dt_code(x.dtype), dt_code(out.dtype), _stream()), "activation")
 
 
 MAX_STREAMS = 16

@@ -74,7 +74,8 @@ class SwiGLU(FeedForward):
 
 class ActMLP(FeedForward):
     """Ungated feed-forward: down(act(up x)), the up product's bias, where there is one, and the activation (the square of
-    relu, or the tanh form of GELU) in that product's epilogue where the kernel takes it, else a pass of their own; the down product's bias is offered to the block."""
+    relu, or the tanh form of GELU) in that product's epilogue where the kernel takes it, else a pass of their own (8 bits: over the float32 sums); the
+    down product's bias is offered to the block."""
 
     def __init__(self, spec, source, rt):
         acts = {"relu2": ops.ACT_RELU2, "gelu_tanh": ops.ACT_GELU_TANH}
@@ -91,8 +92,7 @@ class ActMLP(FeedForward):
     def forward(self, x, ctx, with_bias: bool = True):
         act = torch.empty((x.shape[0], self.up.out_features), device=x.device, dtype=self.rt.dtype)
         if self.up.int8 is not None:
-            self.up(x, out=act)
-            ops.activation(act, act, self.act, bias=self.up_bias)
+            ops.activation(act, self.up(x, out_dtype=torch.float32), self.act, bias=self.up_bias)       # of the sums as they are
         else:
             ops.gemm_act(act, x, self.up.weight, self.up.packed, self.up.out_features, self.act, self.up_bias)
         if self.output_bias is None or not with_bias:
