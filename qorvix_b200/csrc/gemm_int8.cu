@@ -57,7 +57,7 @@ struct Int8Args {
 // stay in L2; grouped: channels fastest, so that they share a tile's rows.
 #define BAND 16
 struct Item { int e, row0, rows, fb; };
-// What the table says of an item (nothing for a dense product), read an item ahead of its use: the trip to memory is then not waited for.
+// What the table says of an item (nothing for a dense product).
 struct Entry { int e, row0, rows; };
 __device__ __forceinline__ Entry entry_of(const Int8Args& p, int item, int items, int NT) {
   Entry n = {-1, 0, 0};
@@ -84,6 +84,36 @@ __device__ __forceinline__ Item item_at(const Int8Args& p, const Entry& n, int i
   it.row0 = (band * BAND + in - it.fb * wide) * p.bn;
   it.rows = p.rows - it.row0 < p.bn ? p.rows - it.row0 : p.bn;
   return it;
+}
+
+// The items of a pair, first, first + pairs, ..., as a warp walks over them: lane l holds the entry of item base + l * pairs, `left` says which of the
+// 32 are still to come.  Entries without an expert or rows are passed over; what comes next is known without a trip to memory, but for one in
+// 32 items (a trip an item, an item ahead: the same times).
+struct Walk { Entry n; int base; unsigned left; };
+__device__ __forceinline__ void look(const Int8Args& p, Walk& w, int items, int pairs, int NT) {
+  const int mine = w.base + pairs * (int)(threadIdx.x & 31);           // (items are 2^30 at most)
+  bool there = mine < items;
+  if (p.tiles) {
+    w.n = entry_of(p, mine, items, NT);
+    there = there && item_at(p, w.n, mine, NT).e >= 0;
+  }
+  w.left = __ballot_sync(0xffffffffu, there);
+}
+__device__ __forceinline__ Item next_item(const Int8Args& p, Walk& w, int items, int pairs, int NT) {       // e -1: there are no more
+  while (!w.left) {
+    w.base += 32 * pairs;
+    if (w.base >= items) return {-1, 0, 0, 0};
+    look(p, w, items, pairs, NT);
+  }
+  const int from = __ffs(w.left) - 1;
+  w.left &= w.left - 1;
+  Entry n = {-1, 0, 0};
+  if (p.tiles) {
+    n.e = __shfl_sync(0xffffffffu, w.n.e, from);
+    n.row0 = __shfl_sync(0xffffffffu, w.n.row0, from);
+    n.rows = __shfl_sync(0xffffffffu, w.n.rows, from);
+  }
+  return item_at(p, n, w.base + pairs * from, NT);
 }
 
 // The gated activations (see GluAct) as g / (1 + exp(-a)) * u: the tanh form of GELU too, 1 + tanh(x) = 2 / (1 + exp(-2 x)), which loses
@@ -169,15 +199,15 @@ __global__ void __launch_bounds__(64 + 32 * pair_epilogue(RT)) int8_pair_kernel(
   pdl_wait();                                        // the rows, the tile table and the output belong to the kernels ahead until here
   const int NT = (p.N + BM - 1) / BM, NP = (NT + 1) / 2, KT = (p.K + QK - 1) / QK;
   const int items = p.row_tiles * NP, first = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  Entry entry = entry_of(p, first, items, NP);
+  Walk walk = {{-1, 0, 0}, first, 0u};
+  look(p, walk, items, pairs, NP);
 
   if (warp == 0) {
     const bool leader = elect_one();
     int it = 0;
     bool ok = true;
-    for (int item = first; ok && item < items; item += pairs) {
-      const Item w = item_at(p, entry, item, NP);
-      entry = entry_of(p, item + pairs, items, NP);
+    while (ok) {
+      const Item w = next_item(p, walk, items, pairs, NP);
       if (w.e < 0) break;
       const int half = ((w.rows + 31) & ~31) >> 1;             // rows of either CTA
       const int boxes = (half + p.box - 1) / p.box;
@@ -204,9 +234,8 @@ __global__ void __launch_bounds__(64 + 32 * pair_epilogue(RT)) int8_pair_kernel(
       const bool leader = elect_one();               // the whole warp walks the loop and waits, an elected lane issues
       int it = 0, local = 0;
       bool ok = true;
-      for (int item = first; ok && item < items; item += pairs, ++local) {
-        const Item w = item_at(p, entry, item, NP);
-        entry = entry_of(p, item + pairs, items, NP);
+      for (; ok; ++local) {
+        const Item w = next_item(p, walk, items, pairs, NP);
         if (w.e < 0) break;
         const uint32_t idesc = umma_idesc_i8(2 * BM, (w.rows + 31) & ~31);
         const int b = local & 1;
@@ -247,11 +276,9 @@ __global__ void __launch_bounds__(64 + 32 * pair_epilogue(RT)) int8_pair_kernel(
         rs[i] = n.e >= 0 && row < n.rows ? p.x_scale[n.row0 + row] : 0.f;
       }
     };
-    Item w = item_at(p, entry, first, NP);
+    Item w = next_item(p, walk, items, pairs, NP);
     fetch(w);
-    entry = entry_of(p, first + pairs, items, NP);
-    int local = 0;
-    for (int item = first; item < items && w.e >= 0; item += pairs, ++local) {
+    for (int local = 0; w.e >= 0; ++local) {
       const int ch0 = (2 * w.fb + rank) * BM + q * 32;         // this warp's channels
       const float w_scale = ws;
       __syncwarp();
@@ -259,11 +286,8 @@ __global__ void __launch_bounds__(64 + 32 * pair_epilogue(RT)) int8_pair_kernel(
       for (int i = 0; i < SCALES / 32; ++i) xs[i * 32 + lane] = rs[i];
       __syncwarp();
       const Item now = w;
-      if (item + pairs < items) {
-        w = item_at(p, entry, item + pairs, NP);
-        fetch(w);
-        entry = entry_of(p, item + 2 * pairs, items, NP);
-      }
+      w = next_item(p, walk, items, pairs, NP);
+      fetch(w);
       const int b = local & 1;
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[b], (local >> 1) & 1, p.err, 63))) break;     // (the MMA warp then gives up too)
       tc_fence_after();

@@ -1986,7 +1986,7 @@ def moe_int8_tile_rows(rows: int, experts: int) -> int:
 def moe_experts_int8(up, out, rows: Int8Rows, weight: Int8Weight, tiles, act: int = GLU_SILU, limit: float = 0.0, slope: float = 0.0, tile_rows: int = 0) -> None:
     """The experts' products in 8-bit integers over rows in grouped order: up True: out [R, N / 2] = act(gate) * up (matrices as for
     gemm_int8_glu), False: out [R, N] the products themselves; float32 or bfloat16.  tiles: moe_group's table, made for tiles of `tile_rows`
-    rows (moe_int8_tile_rows).  Rows that no tile lists are left as they were."""
+    rows (moe_int8_tile_rows); entries that name no expert of these or no rows are passed over.  Rows that no tile lists are left as they were."""
     n = weight.n // 2 if up else weight.n
     R, K = rows.shape
     _i32(tiles, "tiles")
