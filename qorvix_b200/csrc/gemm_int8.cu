@@ -117,8 +117,10 @@ __device__ __forceinline__ Item next_item(const Int8Args& p, Walk& w, int items,
 }
 
 // The gated activations (see GluAct) as g / (1 + exp(-a)) * u: the tanh form of GELU too, 1 + tanh(x) = 2 / (1 + exp(-2 x)), which loses
-// nothing where tanh is near -1.  Where the result is rounded to bfloat16 the fast exponential and quotient serve: their error, a few
-// steps of 2^-23, vanishes in the rounding.
+// nothing where tanh is near -1.  Where the result is rounded to bfloat16 the fast exponential and quotient serve.  The exponential is off by a few
+// steps of 2^-23 and, its argument being scaled to base 2, by |a| of them: under 2^-16 of itself where it is not 0, against the rounding's 2^-9.
+// It is taken of -|a|: it then has no overflow, and the quotient, whose divisor must stay below 2^126, gates as far down as the smallest exponentials
+// (in -103 < a < -87 these have few bits, and 0 below).
 template <typename TO> __device__ __forceinline__ float gated(float g, float u, const GluAct& a) {
   float arg = g;
   if (a.kind == 1) arg = 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
@@ -127,7 +129,10 @@ template <typename TO> __device__ __forceinline__ float gated(float g, float u, 
     u = at_most(at_least(u, -a.limit), a.limit) + 1.f;
     arg = a.slope * g;
   }
-  if (sizeof(TO) == 2) return __fdividef(g, 1.f + __expf(-arg)) * u;
+  if (sizeof(TO) == 2) {
+    const float e = __expf(-fabsf(arg));
+    return __fdividef(arg < 0.f ? g * e : g, 1.f + e) * u;
+  }
   return g / (1.f + expf(-arg)) * u;
 }
 

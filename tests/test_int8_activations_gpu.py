@@ -1,4 +1,4 @@
-"""Activations behind 8-bit products: the float32 sums go into them as they are."""
+"""Activations behind 8-bit products: the float32 sums go into them as they are; gates far below zero keep what bfloat16 can hold of them."""
 from types import SimpleNamespace
 
 import pytest
@@ -57,4 +57,37 @@ def test_ungated_feed_forward(tokens, d, ff, activation, monkeypatch):
     qa, sa = plain.rows(acts[0].cpu())
     down64 = plain.product64(qa, sa, *plain.rows(w["down"]))
     assert ((got.double().cpu() - down64).abs() <= down64.abs() * 2.0 ** -8 + 1e-30).all()
+    ops.check_kernel_errors()
+
+
+@pytest.mark.parametrize("tokens", (1, 40, 300))
+@pytest.mark.parametrize("act", (ops.GLU_SILU, ops.GLU_GELU_TANH, ops.GLU_CLAMPED))
+def test_gates_far_below_zero(act, tokens):
+    """g sigmoid(a) times a large u is an ordinary number where sigmoid(a) is not far above the smallest normal one, 2^-126, and down to the smallest
+    there are: bfloat16 outputs keep it."""
+    f, slope = 512, 1.702
+    ar = torch.linspace(-101.0, -60.0, f, dtype=torch.float64)                 # the exponential's arguments
+    g = ar / slope if act == ops.GLU_CLAMPED else ar
+    if act == ops.GLU_GELU_TANH:                                              # 2 c (g + 0.044715 g^3) = ar, by Newton's method
+        g = torch.full_like(ar, -6.0)
+        for _ in range(60):
+            g = g - (1.5957691216057308 * (g + 0.044715 * g ** 3) - ar) / (1.5957691216057308 * (1 + 3 * 0.044715 * g ** 2))
+    limit = 1e30
+    u = torch.full((f,), 1e30, dtype=torch.float64)
+    z = torch.stack([g.view(-1, 16), u.view(-1, 16)], dim=1).reshape(-1)
+    # one entry a row: the sum is 127 * 127, the token's scale 1 / 127, the channel's the value over 127
+    q = torch.where(z < 0, -127, 127).to(torch.int8).reshape(-1, 1).cuda()
+    s = (z.abs() / 127).float().cuda()
+    x = torch.ones((tokens, 1), device="cuda", dtype=BF16)
+    out = torch.empty((tokens, f), device="cuda", dtype=BF16)
+    ops.gemm_int8_glu(out, x, ops.pack_int8(q, s), act, limit, slope)
+    z64 = plain.product64(*plain.rows(x), q, s)
+    zz = z64.view(tokens, -1, 2, 16)
+    g64, u64 = zz[:, :, 0].reshape(tokens, f), zz[:, :, 1].reshape(tokens, f)
+    a64 = slope * g64 if act == ops.GLU_CLAMPED else 1.5957691216057308 * (g64 + 0.044715 * g64 ** 3) if act == ops.GLU_GELU_TANH else g64
+    e = torch.exp(a64)
+    want = g64 * e / (1 + e) * (u64.clamp(-limit, limit) + 1 if act == ops.GLU_CLAMPED else u64)
+    # as for ordinary gates (16 + 14 |a| steps of 2^-24, half a step of bfloat16), and below the smallest normal exponentials two of their steps
+    bound = want.abs() * (2.0 ** -8 + (16 + 14 * a64.abs()) * 2.0 ** -24) + g64.abs() * u64 * 2.0 ** -148
+    assert ((out.double() - want).abs() <= bound).all()
     ops.check_kernel_errors()
