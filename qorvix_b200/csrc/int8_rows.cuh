@@ -1,7 +1,7 @@
 // Rows in 8-bit integers: q_k = round(127 x_k / top), ties to the even one, and the scale top / 127, with top = max_k |x_k|.
 //   top 0:           scale 0, q 0
 //   top not finite:  scale NaN, q 0 (every product with the row is NaN, as it is in floating arithmetic)
-// The quotient is the exact one: q does not depend on how a kernel forms it.  v = x * (127 / top) in float32 is off by at most 2^-21.8 of itself
+// The quotient is the exact one: q does not depend on how a kernel forms it.  v = x * (127 / top) in float32 is off by at most 2^-21.4 of itself
 // (2^-22 for the quotient of two steps' error that a thread works out for itself, half a step for it as a number, half for the product).
 //   bfloat16 entries: 127 x / top = a / b with whole a up to 127 * 255 and b up to 255, times a power of two; where it is not a half-integer it
 //     differs from every one by 2^-17 of itself or more.  So v rounded to 20 bits (half a step is 2^-21 of it or more, 2^-20 at most) is a
@@ -32,8 +32,9 @@ __device__ __forceinline__ float int8_step(float top) {
 }
 
 // The row's entry x (times s.pre), whose quotient lies next to the border on the side d of the number r that t = r + 1.5 2^23 holds: whether it
-// goes to r or to the next number on that side, as t.  With m = r +- 1/2, 127 x and m top differ by less than 2^-13 of themselves; with p =
-// m top rounded, both 127 x - p and what p was rounded by come out of a multiply-add exactly, so their order is that of the two products.
+// goes to r or to the next number on that side, as t.  With m = r +- 1/2, 127 x and m top differ by less than 2^-12 of themselves (by 1e-4 of a
+// quotient of 1/2 or more); with p = m top rounded, both 127 x - p (fewer than 2^20 units of x's last place) and what p was rounded by come out of
+// a multiply-add exactly, so their order is that of the two products.
 __device__ __forceinline__ float int8_border(float x, float t, float d, float top) {
   const float m = (t - 12582912.f) + copysignf(0.5f, d);
   const float p = m * top, off = fmaf(m, top, -p), a = fmaf(127.f, x, -p);

@@ -425,6 +425,10 @@ int launch_norm_gate(const NormGateArgs& a, int T, int* err, cudaStream_t st) {
   // whole 16-byte pieces in every row that a bulk copy brings
   const bool pieces = ((uintptr_t)a.y & 15) == 0 && ((uintptr_t)a.gate & 15) == 0 && (a.d * sizeof(TY)) % 16 == 0 && (!a.gate || ((a.d * sizeof(TG)) % 16 == 0 && (a.ld_gate * sizeof(TG)) % 16 == 0)) &&
                       (a.ld_y * sizeof(TY)) % 16 == 0;
+  // A block a row up to two rows an SM, where all rows are asked for at once; above, blocks that walk over rows.  us, a block a row / blocks that walk:
+  // bfloat16 y and 8-bit rows, no gate, 150 rows of 2,048 3.0 / 3.3, 600 rows 6.1 / 5.0, 900 rows of 4,096 13.8 / 10.6; with a post norm and a float32 gate,
+  // bfloat16 rows, 150 rows of 2,048 3.8 / 5.8, 600 rows 8.7 / 7.8, 900 rows of 4,096 22.1 / 16.8.  The number at which they are equal falls with the rows'
+  // length (with a gate 1,000 rows of 1,024, 500 of 2,048, 150 of 4,096): 297 to 600 rows of 1,024 lose some 2 us by this rule.
   if (ALIGNED && pieces && T > 2 * sms && a.d <= 8192)
     return fours <= 256    ? launch_norm_gate_rows<TY, TG, OUT, 4, 64>(a, T, sms, err, st)
            : fours <= 640  ? launch_norm_gate_rows<TY, TG, OUT, 4, 160>(a, T, sms, err, st)

@@ -1978,7 +1978,11 @@ def gemm_int8_glu(out, x, weight: Int8Weight, act: int = 0, limit: float = 0.0, 
 
 
 def moe_int8_tile_rows(rows: int, experts: int) -> int:
-    """Rows of a tile of grouped rows for the 8-bit experts' products: what the tile table (moe_group) is made for."""
+    """Rows of a tile of grouped rows for the 8-bit experts' products: what the tile table (moe_group) is made for.  Every tile of an expert reads the
+    expert's matrices, so a tile should hold all rows of a usual expert (4/3 of the mean: counts scatter around it), and no more rows than that,
+    since a pair of SMs takes a whole tile.  us, up / down, tiles of 32, 64, 128, 256 rows, 64 experts of 1,408 x 2,048, 6 a token: 8 tokens 29.9 30.2 30.1
+    30.1 / 15.4 15.2 15.0 15.1; 512 tokens 68.6 63.5 61.4 61.7 / 42.0 37.5 37.2 37.6; 2,048 tokens 182 118 94.1 83.4 / 117 79.6 63.8 60.4.  8 experts of 1,408 x
+    4,096, 2 a token: 32 tokens 20.1 20.6 20.9 21.6 / 11.5 11.2 11.3 11.4; 512 tokens 35.0 24.8 21.9 25.8 / 21.3 16.3 14.3 14.3."""
     want = -(-4 * rows // (3 * max(experts, 1)))
     return 32 if want <= 32 else 64 if want <= 64 else 128 if want <= 128 else 256
 

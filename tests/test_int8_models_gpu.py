@@ -1,5 +1,5 @@
 """Every architecture with its layers' matrices in 8 bits: which products are, and that each of them is the exact one over the 8-bit rows; Tubazen's
-logits against its plain decoder with those products."""
+logits against its plain decoder with those products; and how far 8-bit weights move a decoder's logits."""
 import pytest
 import torch
 
@@ -10,7 +10,9 @@ import lotirax_helpers
 import lugizen_helpers
 import nedasun_helpers
 import plain_tubazen
+import test_int8_engine_gpu as engine
 import tubazen_helpers
+from helpers import PlainModel, make_model_dir, random_tokens
 from qorvix_b200 import ModelRunner, StepEntry
 from qorvix_b200.csrc import ops
 from qorvix_b200.parts import linear
@@ -145,3 +147,19 @@ def test_logits_of_a_model_with_shared_projections(config, small_too):
         rel = d.pow(2).mean(dim=-1).sqrt() / want.pow(2).mean().sqrt()
         assert float(rel.median()) < 0.094 and float(rel.max()) < 0.38, (what, float(rel.median()), float(rel.max()))
     ops.check_kernel_errors()
+
+
+def test_logits_beside_those_of_the_model_as_stored():
+    """A row of 1,024 normal numbers has its largest at 3.3 times their rms: a step is 3.3 / 127 of it and rounding to whole numbers of steps loses a uniform error,
+    its rms 1 / sqrt(12) of a step, 0.75 % of the row's.  Rows and matrix each do that to a product, 1.06 %; eight products of two layers, in squares,
+    3.0 % of the logits' rms.  No more than twice that, and no less than a quarter (or nothing was rounded)."""
+    path = make_model_dir(engine.CFG, seed=4)
+    toks = random_tokens(engine.CFG.vocab_size, 150, 3)
+    ref = PlainModel(path).logits(toks).double()
+    off = {}
+    for weights in ("stored", "int8"):
+        r = ModelRunner(str(path), dtype="bfloat16", max_tokens=512, max_requests=2, weights=weights)
+        got = r.step([StepEntry("w", toks, list(range(150)))], end=["w"]).double().cpu()
+        off[weights] = float((got - ref).pow(2).mean().sqrt() / ref.pow(2).mean().sqrt())
+    print(off)
+    assert 0.0075 < off["int8"] < 0.06 and off["stored"] < off["int8"], off
