@@ -453,8 +453,8 @@ __global__ void __launch_bounds__(std::is_void<TX>::value ? 192 : 64 + FEW_QUANT
       asm volatile("barrier.cluster.arrive.release;" ::: "memory");
       asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     }
+    pdl_wait();                                      // (no bounded wait begins while the kernel ahead is still at work, here or in the warp below)
     if (!INSIDE) {
-      pdl_wait();
       if (leader)
         for (int kb = 0; kb < pre; ++kb) tma_load_2d(ring + kb * STAGE_BYTES + W_TILE_BYTES, &map_x, &full[kb], (kb0 + kb) * QK, row0);
       __syncwarp();
@@ -481,6 +481,7 @@ __global__ void __launch_bounds__(std::is_void<TX>::value ? 192 : 64 + FEW_QUANT
       asm volatile("barrier.cluster.arrive.release;" ::: "memory");
       asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     }
+    pdl_wait();
     const bool there = !INSIDE || mbar_wait(rows_there, 0, p.err, 66);
     for (int kb = 0; there && kb < num_kb; ++kb) {
       const int s = kb % STAGES;
