@@ -278,9 +278,10 @@ __global__ void __launch_bounds__(FOURS == 4 ? 512 : 1024) norm_gate_kernel(cons
 // entries an instruction.  Every row of every operand on 16 bytes and a multiple of them, rows of up to FOURS groups of THREADS threads, as many
 // blocks on an SM as make 640 threads (768 with no gate and no 8-bit rows, which need fewer registers): one block's sums and stores run beside
 // another's.
-// us, 2,048 rows of 5,120, bfloat16 y and gate: bfloat16 rows 27.9 (5.3 TB/s), 8-bit rows 27.9; with two groups a thread and scalar arithmetic 26.8
-// and 34.5 (8,192 rows of 4,096 without a gate: 66.8 and 61.7, so 68.2 and 86.3; 2,048 rows of 2,048: 12.9 and 14.8, so 15.5 and 19.5); 53 with a block
-// a row, which waits for its loads and its sums in turn.
+// us, 2,048 rows of 5,120, bfloat16 y and gate, captured calls over 300 MB in turn: bfloat16 rows 30.0 (4.9 TB/s), 8-bit rows 31.3; 8,192 rows of 4,096
+// without a gate 69.0 and 62.4, 2,048 rows of 2,048 15.3 and 17.4.  Beside two groups a thread and scalar arithmetic, over less memory: 27.9 and 27.9, so
+// 26.8 and 34.5 (8,192 rows of 4,096: 66.8 and 61.7, so 68.2 and 86.3; 2,048 rows of 2,048: 12.9 and 14.8, so 15.5 and 19.5); 53 with a block a row, which
+// waits for its loads and its sums in turn.
 // Two stages or six: 39.9 and 43.2 for rows of 8,192.
 __device__ __forceinline__ float block_total_of(float v, float* red /* >= 32; read by all since this row's or the last row's barrier */) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;

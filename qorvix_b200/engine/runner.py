@@ -45,8 +45,9 @@ class ModelRunner:
                  device="cuda", use_graphs: bool = True, max_graph_batch: int = 64, weights: str = "stored"):
         """model_dir: folder with config.json and model.safetensors; or config + tensors (a
         mapping name -> tensor) for a model held in memory.  max_tokens sizes the page pool.
-        weights: "stored", or "int8" (bfloat16 only): the layers' large matrices are put into 8-bit integers with a scale for each
-        output channel when the model is loaded, and their products run over 8-bit rows with a scale for each token."""
+        weights: "stored", or "int8" (bfloat16 only): the layers' large bfloat16 matrices are put into 8-bit integers with a scale for each
+        output channel when the model is loaded, and their products run over 8-bit rows with a scale for each token (the embedding, the head,
+        ungated experts chosen by a table and what a checkpoint stores in 32 bits stay as stored)."""
         if weights not in WEIGHTS:
             raise ValueError(f"weights must be one of {', '.join(WEIGHTS)}, not {weights!r}")
         if weights == "int8" and parse_dtype(dtype) != torch.bfloat16:
