@@ -69,3 +69,36 @@ def test_tables_without_any_tile():
         ops.moe_experts_int8(False, out, rows, w, table, tile_rows=32)
     assert (out == 9.0).all()
     ops.check_kernel_errors()
+
+
+def test_more_items_than_a_warp_looks_at_in_one_go():
+    """More than 32 items a pair of SMs, of a table with empty entries and of a dense product."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n, k, counts = 4000, 64, (2500, 0, 700, 3333, 1)
+    R = sum(counts)
+    x = torch.randn((R, k), generator=g, device="cuda").to(BF16)
+    q = torch.randint(-127, 128, (len(counts), n, k), generator=g, device="cuda", dtype=torch.int32).to(torch.int8)
+    s = torch.rand((len(counts), n), generator=g, device="cuda") / (64 * k ** 0.5)
+    rows = ops.int8_rows(R, k, "cuda")
+    ops.quantize_rows(rows, x)
+    table, first = [], 0
+    for e, c in enumerate(counts):
+        table += [t for r in range(0, c, 32) for t in ((e, first + r, min(32, c - r)), NONE[r // 32 % len(NONE)])]
+        first += c
+    assert len(table) * 16 > 2 * 32 * 74
+    out = torch.full((R, n), 9.0, device="cuda", dtype=F32)
+    ops.moe_experts_int8(False, out, rows, ops.pack_int8(q, s), torch.tensor(table, dtype=torch.int32, device="cuda").reshape(-1), tile_rows=32)
+    qx, sx = plain.rows(x)
+    at = 0
+    for e, c in enumerate(counts):
+        assert torch.equal(out[at: at + c], plain.product32(qx[at: at + c], sx[at: at + c], q[e], s[e]))
+        at += c
+    x = torch.randn((45000, 32), generator=g, device="cuda").to(BF16)
+    q, s = q[0, :, :32].contiguous(), s[0]
+    out = torch.empty((45000, n), device="cuda", dtype=BF16)
+    ops.gemm_int8(out, x, ops.pack_int8(q, s))
+    qx, sx = plain.rows(x)
+    for part in range(0, 45000, 5000):
+        here = slice(part, part + 5000)
+        assert torch.equal(out[here], plain.product32(qx[here], sx[here], q, s).to(BF16))
+    ops.check_kernel_errors()
